@@ -248,6 +248,144 @@ int vcpp_paged_mixed_step(const vcpp_kv_pages* kv, const float* dq, float* dout,
 size_t vcpp_mixed_workspace_size(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t num_heads,
                                  int32_t max_context_len, int32_t max_blocks_per_chunk);
 
+/* ---- v2: drafted tokens: tree attention and the accepted path ----------- */
+
+/*
+ * Attention of drafted tokens that form a tree, over paged prefixes: what
+ * verifies a step of speculative decoding.  Sequence s owns rows (nodes)
+ * q_start[s] .. q_start[s+1]-1; node i's K/V is at position prefix_lens[s] + i
+ * of its pages (written before the call, with rotary positions of the node's
+ * depth).  Node i attends every position of the prefix and the nodes a whose
+ * bit a is set in its mask row (normally its ancestors and itself).
+ *   q            fp16 (binary16 bits) [total_rows][num_heads][head_dim]
+ *   out          fp32 [total_rows][num_heads][head_dim] (overwritten)
+ *   lse          fp32 [total_rows][num_heads] or NULL: each row's natural
+ *                log-sum-exp of its scaled logits (-inf where it sees nothing)
+ *   block_tables [num_seqs][max_blocks_per_seq] int32
+ *   q_start      [num_seqs + 1] int32 on the device (q_start[0] == 0)
+ *   prefix_lens  [num_seqs] int32 on the device
+ *   tree_mask    [total_rows][mask_words] uint64 on the device, bit a % 64 of
+ *                word a / 64 for node a; NULL: a chain (node i attends nodes
+ *                0 .. i), for one-token decodes and windows of a prompt
+ *   max_nodes    host-side upper bound of the trees' sizes, at most
+ *                VCPP_MAX_TREE_NODES and 64 * mask_words; nodes past it are
+ *                neither attended nor written (a caller error)
+ *   max_prefix_len  host-side upper bound of prefix_lens (sizes the key
+ *                split); positions at or past max_prefix_len + max_nodes are
+ *                not attended
+ *   workspace    device scratch of at least vcpp_tree_workspace_size(...)
+ *                bytes, 16-byte aligned (none needed when that is 0); scratch
+ *                for the call only, so calls that may overlap need separate ones
+ * Semantics as vcpp_paged_decode (missing blocks are skipped; a row that sees
+ * nothing gets zeros); a drafted K or V row that holds inf or NaN reaches only
+ * the rows that attend it.  P is kept to 22 bits: results agree with an fp32
+ * softmax to about 1e-6.  Requirements as vcpp_paged_prefill (fp16, int8 and
+ * FP8 pages; head_dim 64, 80 or 128); total_rows <= num_seqs * max_nodes.
+ * No reference counterpart: the reference decodes one token at a time
+ * (src/paged_engine.cpp:451-550).
+ */
+#define VCPP_MAX_TREE_NODES 256
+int vcpp_paged_tree_attention(const vcpp_kv_pages* kv, const uint16_t* q, float* out, float* lse,
+                              const int32_t* block_tables, int32_t max_blocks_per_seq, const int32_t* q_start,
+                              const int32_t* prefix_lens, const uint64_t* tree_mask, int32_t mask_words,
+                              int32_t num_seqs, int32_t max_nodes, int32_t max_prefix_len, int32_t num_heads,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes vcpp_paged_tree_attention needs for these arguments on the
+ * current device. */
+size_t vcpp_tree_workspace_size(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t max_nodes,
+                                int32_t max_prefix_len, int32_t num_heads);
+
+/*
+ * Moves the rows of an accepted path into place, in every layer: position
+ * prefix_lens[s] + j takes the K/V row (and int8 scales) of position
+ * prefix_lens[s] + accepted[s][j] for j < accept_lens[s], as if all rows were
+ * read before any is written.  The context is then prefix_lens[s] +
+ * accept_lens[s] tokens long.
+ *   kv           the pages of layer 0 (written)
+ *   accepted     [num_seqs][max_accepted] int32 node indices; entries outside
+ *                [0, max_nodes), and rows whose block is missing, move nothing
+ *   accept_lens  [num_seqs] int32 on the device (values past max_accepted
+ *                count as max_accepted)
+ *   max_accepted, max_nodes  1 .. VCPP_MAX_TREE_NODES
+ *   num_layers, layer_stride, scale_layer_stride  the layers' pages are
+ *                layer_stride elements of the KV dtype apart (int8 scales:
+ *                scale_layer_stride fp16 elements); strides unused for 1 layer
+ * Sequences must not share the blocks that hold their trees.  Any page dtype.
+ */
+int vcpp_kv_commit(const vcpp_kv_pages* kv, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                   const int32_t* prefix_lens, const int32_t* accepted, const int32_t* accept_lens,
+                   int32_t num_seqs, int32_t max_accepted, int32_t max_nodes, int32_t num_layers,
+                   int64_t layer_stride, int64_t scale_layer_stride, void* stream);
+
+/* ---- v2: a bounded cache: attention weights, eviction ------------------- */
+
+/*
+ * Adds up the attention that cached positions receive: for every sequence s,
+ * kv head g and position j,
+ *   scores[s][g][j] += sum over rows i and heads h of group g that attend j of
+ *                      exp(q_ih . k_j / sqrt(head_dim) - lse[i][h])
+ * with rows, masks and positions as in vcpp_paged_tree_attention, whose lse
+ * output (for the same queries) is this call's input.  One query per sequence
+ * and no mask: a decode step; a chain of the last queries of a prompt: their
+ * window.
+ *   lse          fp32 [total_rows][num_heads]; a row of -inf adds nothing
+ *   scores       fp32 [num_seqs][num_kv_heads][score_stride], read and written
+ *                at positions < prefix + nodes on valid blocks only;
+ *                score_stride >= max_prefix_len + max_nodes
+ * The sums are formed in fp32 in a fixed order (no atomics).
+ */
+int vcpp_attention_mass(const vcpp_kv_pages* kv, const uint16_t* q, const float* lse, float* scores,
+                        int64_t score_stride, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                        const int32_t* q_start, const int32_t* prefix_lens, const uint64_t* tree_mask,
+                        int32_t mask_words, int32_t num_seqs, int32_t max_nodes, int32_t max_prefix_len,
+                        int32_t num_heads, void* stream);
+
+/*
+ * Plans the cut of every sequence longer than `budget` back to `budget`
+ * positions, per kv head: protected positions stay, then those of the highest
+ * scores (NaN lowest; equal ones in slot order).  Kept rows in front of the
+ * budget stay where they are; the j-th slot there that is given up takes the
+ * j-th kept row behind it.  Attention does not depend on the order of its
+ * positions, so nothing else has to move.
+ *   scores       fp32 [num_seqs][num_kv_heads][stride] (vcpp_attention_mass)
+ *   positions    int32 of the same shape, or NULL: the token position that
+ *                each slot holds; negative: the slot's tokens were appended in
+ *                order and slot j holds position seen - len + j.  Fill it with
+ *                -1 for a new sequence; positions_out keeps it up to date
+ *   context_lens [num_seqs] int32 slots in use (at most max_context_len)
+ *   seen_lens    [num_seqs] int32 tokens the sequence has seen, or NULL (=
+ *                context_lens: nothing was ever evicted)
+ *   keep_first, keep_last  positions < keep_first and >= seen - keep_last are
+ *                protected; their sum is at most budget
+ *   moves        int32 [num_seqs][num_kv_heads][max_moves][2] (to, from),
+ *                entries past the count are left as they are; max_moves >=
+ *                min(budget, max_context_len - budget)
+ *   move_counts  int32 [num_seqs][num_kv_heads]
+ *   new_lens     int32 [num_seqs]: min(context_lens, budget); not context_lens
+ *                itself
+ *   scores_out, positions_out  the state after the moves, slots < new_lens;
+ *                slots new_lens .. max_context_len - 1 become 0 and -1.  They
+ *                may be scores and positions (in place); positions_out may be
+ *                NULL
+ */
+int vcpp_kv_evict_plan(const float* scores, const int32_t* positions, int64_t stride,
+                       const int32_t* context_lens, const int32_t* seen_lens, int32_t num_seqs,
+                       int32_t num_kv_heads, int32_t max_context_len, int32_t budget, int32_t keep_first,
+                       int32_t keep_last, int32_t* moves, int32_t max_moves, int32_t* move_counts,
+                       int32_t* new_lens, float* scores_out, int32_t* positions_out, void* stream);
+
+/*
+ * Moves K/V rows (and int8 scales) inside the pages, per kv head: `moves` and
+ * `move_counts` as vcpp_kv_evict_plan writes them.  No target may be a source
+ * (a plan's never are); moves from or to a missing block are skipped.  The
+ * sequences must not share the blocks in question (copy shared prefixes
+ * first).  Blocks past new_lens are then free to be returned.  Any page dtype.
+ */
+int vcpp_kv_evict_apply(const vcpp_kv_pages* kv, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                        const int32_t* moves, int32_t max_moves, const int32_t* move_counts, int32_t num_seqs,
+                        void* stream);
+
 /* ---- v2: writing K/V into the pages ------------------------------------ */
 
 /*

@@ -289,6 +289,13 @@ int check_pages(const vcpp_kv_pages* kv) {
 
 }  // namespace
 
+namespace vcpp {
+// For the entry points of other sources (api_tree.cpp).
+int check_kv_pages(const vcpp_kv_pages* kv) { return check_pages(kv); }
+void clear_error() { g_last_error.clear(); }
+int compute_units() { return device_cus(); }
+}  // namespace vcpp
+
 // ---- v2: query / key preparation ------------------------------------------
 
 int vcpp_qk_norm_rope(float* q, float* k, int32_t num_tokens, int32_t num_heads,

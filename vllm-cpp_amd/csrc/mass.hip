@@ -1,0 +1,187 @@
+// mass.hip -- the softmax weights of a step's queries, added up per kv head
+// and cache position: scores[s][g][j] += sum over the rows (node i, head h of
+// group g) that see position j of exp(q_i . k_j / sqrt(D) - lse_i).
+//
+// With the rows' log-sum-exp given, every position is independent: no running
+// maximum, no merge, and each sum is formed by one wave in a fixed order (no
+// atomics, the same bits every time).  A wave owns KT tiles of 16 positions;
+// S[16 rows][16 positions] = Q x K^T comes from 16x16x32 f16 products with the
+// rows along a lane's accumulators, so that a lane sums its position's weights
+// in registers and only the four lane groups meet at the end.  K goes straight
+// from its pages to the product's operands (a lane's 16 bytes are 16 bytes of
+// its position's row): each row of K is read once per kv head.
+#include "device_common.h"
+#include "tree.h"
+#include "tree_mask.h"
+
+namespace vcpp {
+
+namespace {
+
+constexpr int kMassTiles = 4;                   // 16-position tiles of a wave
+constexpr int kMassKeys = 16 * kMassTiles;      // positions of a wave
+constexpr int kMassWaves = 4;
+
+// Operand k slices of a row: 8 dims of lane group g in slice i.  fp16 pages:
+// dims 32 i + 8 g.  Byte pages: 16 consecutive bytes of a lane serve two
+// slices.  A 16-dim rest (D = 80) fills lane groups 0 and 1 of a last slice.
+template <int KV, int D>
+struct MassDims {
+    static constexpr int NC = D / 32, REM = (D % 32) / 16, NS = NC + REM;
+    __device__ static __forceinline__ int dim(int i, int g) {
+        if (i == NC) return 32 * NC + 8 * g;  // (g < 2)
+        return KV == VCPP_KV_F16 ? 32 * i + 8 * g : 64 * (i >> 1) + 16 * g + 8 * (i & 1);
+    }
+};
+
+template <int KV, int D>
+__device__ __forceinline__ void load_k(const TreeParams& p, int64_t row, int g, h8 (&k)[MassDims<KV, D>::NS]) {
+    using M = MassDims<KV, D>;
+    if constexpr (KV == VCPP_KV_F16) {
+        const _Float16* b = static_cast<const _Float16*>(p.k) + row;
+#pragma unroll
+        for (int i = 0; i < M::NS; ++i)
+            k[i] = i < M::NC || g < 2 ? *reinterpret_cast<const h8*>(b + M::dim(i, g)) : h8{};
+    } else {
+        const uint8_t* b = static_cast<const uint8_t*>(p.k) + row;
+#pragma unroll
+        for (int i = 0; i < M::NC; i += 2) {
+            const i4 x = *reinterpret_cast<const i4*>(b + M::dim(i, g));
+            k[i] = bytes8_to_h8<KV>((uint32_t)x.x, (uint32_t)x.y);
+            k[i + 1] = bytes8_to_h8<KV>((uint32_t)x.z, (uint32_t)x.w);
+        }
+        if constexpr (M::REM) {
+            i2 x = {0, 0};
+            if (g < 2) x = *reinterpret_cast<const i2*>(b + M::dim(M::NC, g));
+            k[M::NC] = g < 2 ? bytes8_to_h8<KV>((uint32_t)x.x, (uint32_t)x.y) : h8{};
+        }
+    }
+}
+
+template <int KV, int D>
+__global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
+    using MD = MassDims<KV, D>;
+    constexpr bool SCALED = KV == VCPP_KV_I8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    // The kv heads of one (sequence, part) share an XCD (and its L2's lines).
+    const int jj = blockIdx.x >> 3;
+    const int cell = (jj / p.num_kv_heads) * 8 + (blockIdx.x & 7);
+    const int kvh = jj % p.num_kv_heads;
+    const int part = cell / p.num_seqs, s = cell - part * p.num_seqs;
+    if (part >= p.parts) return;
+    const TreeSeq sq(p, s);
+    const int G = p.group, M = sq.n * G;
+    const int k_hi = min(part * p.part_len + p.part_len, sq.end);
+    if (M == 0) return;
+    const int32_t* table = p.block_tables + (int64_t)s * p.max_blocks;
+    float* out = p.scores + ((int64_t)s * p.num_kv_heads + kvh) * p.score_stride;
+
+    for (int k0 = part * p.part_len + kMassKeys * wave; k0 < k_hi; k0 += kMassKeys * kMassWaves) {
+        h8 k[kMassTiles][MD::NS];
+        float ksc[kMassTiles];
+        bool ok[kMassTiles];
+#pragma unroll
+        for (int kt = 0; kt < kMassTiles; ++kt) {
+            const int pos = k0 + 16 * kt + c;
+            const int lb = (int)(((uint64_t)(uint32_t)pos * p.bs_magic) >> 40);
+            const int bid = pos < k_hi && lb < p.max_blocks ? table[lb] : -1;
+            ok[kt] = bid >= 0 && (int64_t)bid < p.num_blocks;
+            const int slot = pos - lb * p.block_size;
+            ksc[kt] = p.scale_log2;
+            if (ok[kt]) {
+                load_k<KV, D>(p, (int64_t)bid * p.block_stride + ((int64_t)slot * p.num_kv_heads + kvh) * D, g, k[kt]);
+                if constexpr (SCALED)
+                    ksc[kt] *= (float)__builtin_bit_cast(
+                        _Float16, p.k_scale[(int64_t)bid * p.scale_block_stride + (int64_t)kvh * p.block_size + slot]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < MD::NS; ++i) k[kt][i] = h8{};
+            }
+        }
+        const bool masked = k0 + kMassKeys > sq.prefix;
+        float sum[kMassTiles] = {0.f, 0.f, 0.f, 0.f};
+        for (int r0 = 0; r0 < M; r0 += 16) {
+            h8 q[MD::NS];
+            {
+                const int row = r0 + c, t = row / G;
+                const bool in = row < M;
+                const _Float16* b = reinterpret_cast<const _Float16*>(p.q) +
+                                    ((int64_t)(sq.q0 + (in ? t : 0)) * p.num_heads + kvh * G + (in ? row - t * G : 0)) * D;
+#pragma unroll
+                for (int i = 0; i < MD::NS; ++i)
+                    q[i] = in && (i < MD::NC || g < 2) ? *reinterpret_cast<const h8*>(b + MD::dim(i, g)) : h8{};
+            }
+            float shift[4];
+            uint64_t win[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = r0 + 4 * g + r, t = row / G;
+                shift[r] = __builtin_inff();  // (rows past the last, and rows that saw nothing, add exp2(-inf))
+                win[r] = 0;
+                if (row < M) {
+                    const float z = p.lse_in[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)];
+                    if (z != -__builtin_inff()) shift[r] = z * kLog2e;
+                    if (masked) {
+                        const uint64_t* mrow = p.mask ? p.mask + (int64_t)(sq.q0 + t) * p.mask_words : nullptr;
+                        win[r] = (uint64_t)tree_window(p, sq, mrow, t, k0 + 32) << 32 | tree_window(p, sq, mrow, t, k0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int kt = 0; kt < kMassTiles; ++kt) {
+                f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < MD::NS; ++i) acc = mfma32(q[i], k[kt][i], acc);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = fmaf(acc[r], ksc[kt], -shift[r]);
+                    if (masked) x = (win[r] >> (16 * kt + c)) & 1 ? x : -__builtin_inff();
+                    sum[kt] += fast_exp2(x);
+                }
+            }
+        }
+        // The four lane groups' sums; group g writes tile g.
+        float mine = 0.f;
+        bool write = false;
+#pragma unroll
+        for (int kt = 0; kt < kMassTiles; ++kt) {
+            float x = sum[kt];
+            x += shfl_xor(x, 32);
+            x += shfl_xor(x, 16);
+            if (g == kt) mine = x, write = ok[kt];
+        }
+        if (write) out[k0 + lane] += mine;
+    }
+}
+
+template <int KV, int D>
+hipError_t launch_mass_dim(const TreeParams& p, hipStream_t stream) {
+    const int64_t cells = (int64_t)p.num_seqs * p.parts;
+    const int64_t grid = (cells + 7) / 8 * 8 * p.num_kv_heads;
+    mass_kernel<KV, D><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <int KV>
+hipError_t launch_mass_kv(const TreeParams& p, hipStream_t stream) {
+    switch (p.head_dim) {
+        case 64: return launch_mass_dim<KV, 64>(p, stream);
+        case 80: return launch_mass_dim<KV, 80>(p, stream);
+        case 128: return launch_mass_dim<KV, 128>(p, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_mass(const TreeParams& p, hipStream_t stream) {
+    switch (p.kv_dtype) {
+        case VCPP_KV_F16: return launch_mass_kv<VCPP_KV_F16>(p, stream);
+        case VCPP_KV_I8: return launch_mass_kv<VCPP_KV_I8>(p, stream);
+        case VCPP_KV_FP8: return launch_mass_kv<VCPP_KV_FP8>(p, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace vcpp

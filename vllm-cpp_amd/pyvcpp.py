@@ -41,6 +41,12 @@ EXPORTS = [
     "flash_attention_cuda",
     "vcpp_profile_enable",
     "vcpp_profile_read",
+    "vcpp_tree_workspace_size",
+    "vcpp_paged_tree_attention",
+    "vcpp_attention_mass",
+    "vcpp_kv_commit",
+    "vcpp_kv_evict_plan",
+    "vcpp_kv_evict_apply",
 ]
 
 KERNEL_DECODE, KERNEL_MERGE, KERNEL_PREFILL, KERNEL_MIXED = 0, 1, 2, 3
@@ -119,6 +125,21 @@ def open_library(path):
     L.vcpp_mixed_workspace_size.restype = sz
     L.vcpp_write_kv.argtypes = [ctypes.POINTER(KVPages), vp, vp, vp, i32, i32, vp]
     L.vcpp_write_kv.restype = ctypes.c_int
+    L.vcpp_tree_workspace_size.argtypes = [ctypes.POINTER(KVPages), i32, i32, i32, i32]
+    L.vcpp_tree_workspace_size.restype = sz
+    L.vcpp_paged_tree_attention.argtypes = [ctypes.POINTER(KVPages), vp, vp, vp, vp, i32, vp, vp, vp, i32, i32,
+                                            i32, i32, i32, vp, sz, vp]
+    L.vcpp_paged_tree_attention.restype = ctypes.c_int
+    L.vcpp_attention_mass.argtypes = [ctypes.POINTER(KVPages), vp, vp, vp, i64, vp, i32, vp, vp, vp, i32, i32,
+                                      i32, i32, i32, vp]
+    L.vcpp_attention_mass.restype = ctypes.c_int
+    L.vcpp_kv_commit.argtypes = [ctypes.POINTER(KVPages), vp, i32, vp, vp, vp, i32, i32, i32, i32, i64, i64, vp]
+    L.vcpp_kv_commit.restype = ctypes.c_int
+    L.vcpp_kv_evict_plan.argtypes = [vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp,
+                                     vp]
+    L.vcpp_kv_evict_plan.restype = ctypes.c_int
+    L.vcpp_kv_evict_apply.argtypes = [ctypes.POINTER(KVPages), vp, i32, vp, i32, vp, i32, vp]
+    L.vcpp_kv_evict_apply.restype = ctypes.c_int
     L.vcpp_qk_norm_rope.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp, ctypes.c_float, vp, vp,
                                     i32, i32, vp]
     L.vcpp_qk_norm_rope.restype = ctypes.c_int
@@ -281,6 +302,112 @@ def paged_prefill_split(pages, q, out, block_tables, q_start, prefix_lens, max_c
                                         _stream(stream))
     _check(rc)
     return out
+
+
+def _operand(name, t, dtype, shape=None):
+    """Address of a dense tensor of this dtype (and shape) on the current
+    device; anything else would be misread."""
+    import torch
+    if t.dtype is not dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError("%s must be a contiguous %s tensor%s, got %s %s with strides %s" % (
+            name, dtype, " of shape %s" % (shape,) if shape else "", t.dtype, tuple(t.shape), t.stride()))
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError("%s is on %s, not on the current GPU" % (name, t.device))
+    return t.data_ptr()
+
+
+def tree_workspace_size(pages, num_seqs, max_nodes, max_prefix_len, num_heads):
+    return lib().vcpp_tree_workspace_size(ctypes.byref(pages), num_seqs, max_nodes, max_prefix_len, num_heads)
+
+
+def _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens, tree_mask, num_heads):
+    """Checked addresses of what the tree calls share."""
+    import torch
+    rows, S = q.shape[0], prefix_lens.shape[0]
+    words = 0 if tree_mask is None else tree_mask.shape[-1]
+    mask = None if tree_mask is None else _operand("tree_mask", tree_mask, torch.int64, (rows, words))
+    z = None if lse is None else _operand("lse", lse, torch.float32, (rows, num_heads))
+    return (_operand("q", q, torch.float16, (rows, num_heads, pages.head_dim)), z,
+            _operand("block_tables", block_tables, torch.int32, (S, block_tables.shape[-1])), block_tables.shape[-1],
+            _operand("q_start", q_start, torch.int32, (S + 1,)), _operand("prefix_lens", prefix_lens, torch.int32, (S,)),
+            mask, words, S)
+
+
+def paged_tree_attention(pages, q, out, block_tables, q_start, prefix_lens, max_nodes, max_prefix_len, num_heads,
+                         tree_mask=None, lse=None, workspace=None, stream=None):
+    """vcpp_paged_tree_attention: q fp16 [rows][H][D], out fp32 [rows][H][D],
+    lse fp32 [rows][H] or None, tree_mask int64 [rows][words] (the words' bits)
+    or None for chains."""
+    import torch
+    qp, lp, bt, mb, st, pf, mask, words, S = _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens,
+                                                            tree_mask, num_heads)
+    o = _operand("out", out, torch.float32, tuple(q.shape))
+    if q.shape[0] > S * max_nodes:
+        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (q.shape[0], S, max_nodes))
+    if workspace is None:
+        need = tree_workspace_size(pages, S, max_nodes, max_prefix_len, num_heads)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    ws, nbytes = (None, 0) if workspace is None else (_operand("workspace", workspace, torch.uint8), workspace.numel())
+    _check(lib().vcpp_paged_tree_attention(ctypes.byref(pages), qp, o, lp, bt, mb, st, pf, mask, words, S, max_nodes,
+                                           max_prefix_len, num_heads, ws, nbytes, _stream(stream)))
+    return out
+
+
+def attention_mass(pages, q, lse, scores, block_tables, q_start, prefix_lens, max_nodes, max_prefix_len, num_heads,
+                   tree_mask=None, stream=None):
+    """vcpp_attention_mass: adds to scores fp32 [S][Hkv][stride] in place."""
+    import torch
+    qp, lp, bt, mb, st, pf, mask, words, S = _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens,
+                                                            tree_mask, num_heads)
+    if q.shape[0] > S * max_nodes:
+        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (q.shape[0], S, max_nodes))
+    stride = scores.shape[-1]
+    sc = _operand("scores", scores, torch.float32, (S, pages.num_kv_heads, stride))
+    _check(lib().vcpp_attention_mass(ctypes.byref(pages), qp, lp, sc, stride, bt, mb, st, pf, mask, words, S, max_nodes,
+                                     max_prefix_len, num_heads, _stream(stream)))
+    return scores
+
+
+def kv_evict_plan(scores, context_lens, max_context_len, budget, moves, move_counts, new_lens, scores_out,
+                  keep_first=0, keep_last=0, seen_lens=None, positions=None, positions_out=None, stream=None):
+    """vcpp_kv_evict_plan: scores fp32 [S][Hkv][stride] (and positions int32)
+    to moves int32 [S][Hkv][n][2], move_counts [S][Hkv], new_lens [S] and the
+    state after the moves."""
+    import torch
+    S, hkv, stride = scores.shape
+    i32, shape = torch.int32, (S, hkv, stride)
+    _check(lib().vcpp_kv_evict_plan(
+        _operand("scores", scores, torch.float32), None if positions is None else _operand("positions", positions, i32, shape),
+        stride, _operand("context_lens", context_lens, i32, (S,)),
+        None if seen_lens is None else _operand("seen_lens", seen_lens, i32, (S,)), S, hkv, max_context_len, budget,
+        keep_first, keep_last, _operand("moves", moves, i32, (S, hkv, moves.shape[2], 2)), moves.shape[2],
+        _operand("move_counts", move_counts, i32, (S, hkv)), _operand("new_lens", new_lens, i32, (S,)),
+        _operand("scores_out", scores_out, torch.float32, shape),
+        None if positions_out is None else _operand("positions_out", positions_out, i32, shape), _stream(stream)))
+
+
+def kv_evict_apply(pages, block_tables, moves, move_counts, stream=None):
+    """vcpp_kv_evict_apply: the planned row moves inside the pages."""
+    import torch
+    S, blocks = block_tables.shape
+    n = moves.shape[2]
+    _check(lib().vcpp_kv_evict_apply(
+        ctypes.byref(pages), _operand("block_tables", block_tables, torch.int32), blocks,
+        _operand("moves", moves, torch.int32, (S, pages.num_kv_heads, n, 2)), n,
+        _operand("move_counts", move_counts, torch.int32, (S, pages.num_kv_heads)), S, _stream(stream)))
+
+
+def kv_commit(pages, block_tables, prefix_lens, accepted, accept_lens, max_nodes, num_layers=1, layer_stride=0,
+              scale_layer_stride=0, stream=None):
+    """vcpp_kv_commit: accepted int32 [S][n] node indices, accept_lens int32 [S]."""
+    import torch
+    S, blocks = block_tables.shape
+    n = accepted.shape[1]
+    _check(lib().vcpp_kv_commit(
+        ctypes.byref(pages), _operand("block_tables", block_tables, torch.int32), blocks,
+        _operand("prefix_lens", prefix_lens, torch.int32, (S,)), _operand("accepted", accepted, torch.int32, (S, n)),
+        _operand("accept_lens", accept_lens, torch.int32, (S,)), S, n, max_nodes, num_layers, layer_stride,
+        scale_layer_stride, _stream(stream)))
 
 
 def write_kv(pages, k, v, slots, fp16_round_nearest=False, stream=None):
