@@ -25,8 +25,8 @@ namespace {
 static_assert(vcpp::kMaxTreeNodes == VCPP_MAX_TREE_NODES, "tree size");
 
 // Longest context of these calls: pos / block_size as a product (tree.h) stays
-// below 2^63.
-constexpr int64_t kMaxLen = 1 << 26;
+// below 2^63, and 64 sequences' key blocks below 2^31.
+constexpr int64_t kMaxLen = 1 << 24;
 
 int fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -41,33 +41,34 @@ int hip_fail(hipError_t e, const char* what) { return fail(VCPP_E_HIP, "%s: %s",
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Key split of a tree call: parts of part_len positions, and the partials'
-// place in the workspace.
+// Cut of a tree call (TreeRanges) and the partials' place in the workspace.
 struct TreeSplit {
-    int32_t part_len, parts, row_tiles;
+    int32_t ranges, table_cap;
     size_t off_ml, bytes;
 };
 
-// Parts of a call: enough workgroups to fill the GPU about twice where the
-// trees alone do not, each part at least 4 key blocks and at most 16384
-// positions (its block ids live in LDS).
+// Ranges: one per workgroup (and kv head) that the GPU holds at once, fewer
+// where the bounds allow fewer than kTreeMinBlocks blocks each, more where a
+// range's block ids would pass kMaxTable.
+constexpr int64_t kMaxTable = 2048;
+
 TreeSplit tree_split(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t max_nodes, int32_t max_prefix_len,
                      int32_t num_heads) {
     TreeSplit t{};
-    const int group = num_heads / kv->num_kv_heads;
-    const int rows = max_nodes * group;
+    const int rows = max_nodes * (num_heads / kv->num_kv_heads);
     const int tile = vcpp::tree_tile_rows(kv->dtype, kv->head_dim, rows);
-    t.row_tiles = (rows + tile - 1) / tile;
-    const int64_t len = (int64_t)max_prefix_len + max_nodes;
-    const int64_t items = (int64_t)num_seqs * kv->num_kv_heads * t.row_tiles;
-    const int64_t slots = 2 * (int64_t)vcpp::compute_units() * vcpp::tree_wgs_per_cu(kv->dtype, kv->head_dim, rows);
-    const int64_t want = std::max<int64_t>(1, (slots + items - 1) / items);
-    int64_t part = (len + want - 1) / want;
-    part = std::min<int64_t>(std::max<int64_t>(128, (part + 31) / 32 * 32), 16384);
-    t.part_len = (int32_t)part;
-    t.parts = (int32_t)((len + part - 1) / part);
-    if (t.parts > 1) {
-        const size_t n = (size_t)t.parts * num_seqs * max_nodes * num_heads;
+    const int64_t blocks = ((int64_t)max_prefix_len + max_nodes + 31) / 32;
+    const int64_t most = (int64_t)num_seqs * ((rows + tile - 1) / tile) * blocks;  // upper bound of the axis
+    const int64_t slots = (int64_t)vcpp::compute_units() * vcpp::tree_wgs_per_cu(kv->dtype, kv->head_dim, rows);
+    int64_t R = std::min(std::max<int64_t>(1, slots / kv->num_kv_heads), std::max<int64_t>(1, most / vcpp::kTreeMinBlocks));
+    // (a piece is no longer than its sequence, nor than its range)
+    const int64_t per_range = kMaxTable * kv->block_size / 32 - 4;
+    if (blocks > per_range) R = std::max(R, (most + per_range - 1) / per_range);
+    t.ranges = (int32_t)std::min<int64_t>(R, INT32_MAX);
+    const int64_t longest = std::min(blocks, std::max<int64_t>((most + R - 1) / R, 2 * vcpp::kTreeMinBlocks) + 1);
+    t.table_cap = (int32_t)(longest * 32 / kv->block_size + 2);
+    if (t.ranges > 1) {
+        const size_t n = (size_t)t.ranges * 2 * kv->num_kv_heads * tile;
         t.off_ml = align256(n * kv->head_dim * sizeof(float));
         t.bytes = t.off_ml + align256(n * sizeof(float2));
     }
@@ -192,8 +193,7 @@ int vcpp_paged_tree_attention(const vcpp_kv_pages* kv, const uint16_t* q, float*
     if (!out) return fail(VCPP_E_INVALID, "out is NULL");
     if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return fail(VCPP_E_INVALID, "out must be 16-byte aligned");
     const TreeSplit t = tree_split(kv, num_seqs, max_nodes, max_prefix_len, num_heads);
-    if (!grid_fits((int64_t)num_seqs * t.parts, (int64_t)kv->num_kv_heads * t.row_tiles, 256) ||
-        !grid_fits((int64_t)num_seqs * max_nodes, 1, 256))
+    if (!grid_fits(t.ranges, kv->num_kv_heads, 256) || !grid_fits((int64_t)num_seqs * max_nodes, 1, 256))
         return fail(VCPP_E_UNSUPPORTED, "too many sequences, heads or positions for one launch");
     if (t.bytes > 0 && (!workspace || workspace_bytes < t.bytes))
         return fail(VCPP_E_WORKSPACE, "tree attention needs %zu workspace bytes, got %zu", t.bytes,
@@ -204,9 +204,8 @@ int vcpp_paged_tree_attention(const vcpp_kv_pages* kv, const uint16_t* q, float*
                                      mask_words, num_seqs, max_nodes, max_prefix_len, num_heads);
     p.out = out;
     p.lse = lse;
-    p.part_len = t.part_len;
-    p.parts = t.parts;
-    p.row_tiles = t.row_tiles;
+    p.ranges = t.ranges;
+    p.table_cap = t.table_cap;
     if (t.bytes > 0) {
         p.ws_o = static_cast<float*>(workspace);
         p.ws_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + t.off_ml);

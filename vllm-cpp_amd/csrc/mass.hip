@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
                 for (int i = 0; i < MD::NS; ++i) k[kt][i] = h8{};
             }
         }
-        const bool masked = k0 + kMassKeys > sq.prefix;
+        const bool masked = k0 + kMassKeys > sq.plain;
         float sum[kMassTiles] = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < M; r0 += 16) {
             h8 q[MD::NS];

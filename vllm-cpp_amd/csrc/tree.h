@@ -44,18 +44,25 @@ struct TreeParams {
     // attention: fp32 outputs, and each row's log-sum-exp (NULL: none)
     float* out;
     float* lse;
-    int32_t part_len;  // positions per key part (a multiple of 32)
-    int32_t parts;     // most key parts of a sequence (1: no merge)
-    int32_t row_tiles; // row tiles of max_nodes * group rows
+    // Key split (attention): the units (sequence, row tile), each as long as its
+    // key blocks, are cut into `ranges` equal ranges (TreeRanges).
+    int32_t ranges;
+    int32_t table_cap; // block ids of a range's longest piece
     int64_t rows_cap;  // num_seqs * max_nodes
-    float* ws_o;       // [parts][rows_cap][num_heads][head_dim]
-    float2* ws_ml;     // [parts][rows_cap][num_heads] (exponent in log2 units, sum)
+    float* ws_o;       // [ranges][2][num_kv_heads][tile rows][head_dim]
+    float2* ws_ml;     // [ranges][2][num_kv_heads][tile rows] (exponent in log2 units, sum)
+    // Position split (weights): parts of part_len positions.
+    int32_t part_len;
+    int32_t parts;
     // weights: each row's log-sum-exp and the sums [num_seqs][num_kv_heads][score_stride]
     const float* lse_in;
     float* scores;
     int64_t score_stride;
 };
 
+// Key blocks (32 positions) of a range, at least: a call that has fewer is cut
+// into fewer ranges.
+constexpr int kTreeMinBlocks = 4;
 // Rows (node, head of the group) of one workgroup for trees of `rows` rows.
 int tree_tile_rows(int kv_dtype, int head_dim, int rows);
 // Workgroups of that tile a CU holds at once.

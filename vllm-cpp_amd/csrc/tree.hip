@@ -37,7 +37,18 @@ constexpr float kHead = 11.f;         // log2 of the P that a row's running maxi
 constexpr float kTopP = 32768.f;      // 2^15: largest P
 constexpr float kTopLog = 15.f;
 
-typedef uint16_t us8 __attribute__((ext_vector_type(8)));
+
+// Natural log-sum-exp of a row of exponent m (log2 units) and sum l.
+__device__ __forceinline__ float row_lse(float m, float l) {
+    return l == 0.f ? -__builtin_inff() : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
+// x where bit b of w is set, else -inf: a select on integers (compares would
+// hold a pair of scalar registers for every element of a block).
+__device__ __forceinline__ float seen_or_inf(float x, uint32_t w, int b) {
+    const int m = __builtin_amdgcn_sbfe((int)w, b, 1);
+    return __int_as_float((__float_as_int(x) & m) | ((int)0xFF800000u & ~m));
+}
 
 template <int KV, int D, int RB_, int WR_, int ST>
 struct TreeDims {
@@ -54,7 +65,12 @@ struct TreeDims {
     static constexpr int AREA = STAGES * RSTAGE;
     static constexpr int NF16 = !BYTES ? STAGES : WR > 1 ? 2 : 1;  // fp16 blocks
     static constexpr int F16BASE = BYTES ? AREA : 0;
-    static constexpr int TABLE = AREA + (BYTES ? NF16 * DD::STAGE : 0);
+    // Marks of drafted V values that are not finite (not int8): [0] any in this
+    // piece, [1] any in this block, then a 32-key word per dim, then a bit per
+    // (row, dim) of the tile.
+    static constexpr int DW = (D + 31) / 32;
+    static constexpr int MARKS = AREA + (BYTES ? NF16 * DD::STAGE : 0);
+    static constexpr int TABLE = MARKS + (SCALED ? 0 : (2 + D + ROWS * DW) * 4);
     static_assert(STAGES >= 3 && (STAGES - 1) * PERW < 64, "ring depth");
 };
 
@@ -70,8 +86,17 @@ __device__ __forceinline__ void tree_barrier() {
     else asm volatile("" ::: "memory");  // one wave: its LDS accesses are in order
 }
 
+#ifndef T_OCC
+#define T_OCC 2
+#endif
+#ifndef T_RB
+#define T_RB 2
+#endif
+#ifndef T_ST
+#define T_ST 4
+#endif
 template <int KV, int D, int RB, int WR, int ST>
-__global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
+__global__ __launch_bounds__(64 * WR, T_OCC) void tree_kernel(TreeParams p) {
     using T = TreeDims<KV, D, RB, WR, ST>;
     using DD = typename T::DD;
     using ID = typename T::ID;
@@ -82,37 +107,53 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
     const uint32_t lds_addr = (uint32_t)(uintptr_t)lds;
     __attribute__((address_space(3))) int32_t* table_s =
         reinterpret_cast<__attribute__((address_space(3))) int32_t*>(lds + T::TABLE);
+    __attribute__((address_space(3))) uint32_t* marks =
+        reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(lds + T::MARKS);
+    __attribute__((address_space(3))) uint32_t* bad_dims = marks + 2;
+    __attribute__((address_space(3))) uint32_t* bad_outs = bad_dims + D;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    // Consecutive workgroups go to the 8 XCDs in turn: the kv heads and row
-    // tiles of one (sequence, part) share an XCD, whose L2 then holds the
-    // lines that neighbouring heads' rows share.
-    const int per = p.num_kv_heads * p.row_tiles;
+    // Consecutive workgroups go to the 8 XCDs in turn: the kv heads of one
+    // range share an XCD, whose L2 then holds the lines that neighbouring
+    // heads' rows share.
     const int jj = blockIdx.x >> 3;
-    const int cell = (jj / per) * 8 + (blockIdx.x & 7);
-    const int within = jj % per;
-    const int part = cell / p.num_seqs, s = cell - part * p.num_seqs;
-    if (part >= p.parts) return;  // whole workgroup
-    const int kvh = within / p.row_tiles, rt = within - kvh * p.row_tiles;
+    const int kvh = jj % p.num_kv_heads;
+    const int range = (jj / p.num_kv_heads) * 8 + (blockIdx.x & 7);
+    const TreeRanges cut(p, T::ROWS, lane);
+    if (range >= cut.R || cut.total == 0) return;  // whole workgroup
+    const int64_t lo = cut.start(range), hi = cut.start(range + 1);
+    int64_t first;  // first block of sequence s
+    int s = cut.seq_of(p, T::ROWS, lane, lo, first);
+    const int G = p.group;
+    int64_t at_block = lo;
+    while (at_block < hi) {  // the range's pieces, one per unit
     const TreeSeq sq(p, s);
-    const int G = p.group, M = sq.n * G;
+    const int M = sq.n * G;
+    const int tiles = (M + T::ROWS - 1) / T::ROWS, blocks = (sq.end + 31) / 32;
+    if (at_block >= first + (int64_t)tiles * blocks) {  // next sequence
+        first += (int64_t)tiles * blocks;
+        ++s;
+        continue;
+    }
+    const int rt = (int)((at_block - first) / blocks);
+    const int64_t unit0 = first + (int64_t)rt * blocks;  // the unit's first block
+    const int kb_lo = (int)(at_block - unit0);
+    const int kb_hi = (int)min((int64_t)blocks, hi - unit0);
+    const bool whole = kb_lo == 0 && kb_hi == blocks;
+    const int64_t piece = (int64_t)range * 2 + (at_block > lo ? 1 : 0);  // partials' place (not whole)
+    at_block = unit0 + kb_hi;
     const int row0 = rt * T::ROWS;
-    const int k_lo = part * p.part_len;
-    if (row0 >= M || (part > 0 && k_lo >= sq.end)) return;  // whole workgroup
-    const int k_hi = min(k_lo + p.part_len, sq.end);
-    const int kb_lo = k_lo / kKBlk, kb_hi = (k_hi + kKBlk - 1) / kKBlk;
+    const int k_lo = kb_lo * kKBlk, k_hi = min(kb_hi * kKBlk, sq.end);
 
     // Q fragments (B operand): row row0 + 16 (RB wave + rb) + c
     h8 qa[RB][NC32 > 0 ? NC32 : 1];
     h8 qr[RB];
-    int node[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int row = row0 + 16 * (RB * wave + rb) + c;
         const bool ok = row < M;
         const int t = ok ? row / G : 0;
-        node[rb] = ok ? t : -1;
         const _Float16* qrow = reinterpret_cast<const _Float16*>(p.q) +
                                ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (ok ? row - t * G : 0)) * D;
 #pragma unroll
@@ -122,10 +163,12 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
     }
     if (tid < T::NF16)
         *reinterpret_cast<__attribute__((address_space(3))) h8*>(lds + T::F16BASE + tid * DD::STAGE + DD::ZERO) = h8{};
-    // The part's block ids (-1: missing or outside the pool).
+    if constexpr (!SCALED)
+        for (int i = tid; i < 2 + D + T::ROWS * T::DW; i += 64 * WR) marks[i] = 0;
+    // The piece's block ids (-1: missing or outside the pool).
     const int32_t* table = p.block_tables + (int64_t)s * p.max_blocks;
     const int lb0 = k_lo / p.block_size;
-    const int npages = k_hi > k_lo ? (k_hi - 1) / p.block_size + 1 - lb0 : 0;
+    const int npages = min((k_hi - 1) / p.block_size + 1 - lb0, p.table_cap);
     int bad = 0;
     for (int i = tid; i < npages; i += 64 * WR) {
         const int bid = lb0 + i < p.max_blocks ? table[lb0 + i] : -1;
@@ -192,7 +235,7 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
             }
         }
         lds_char* dst0 = lds + T::AREA + (kb % T::NF16) * DD::STAGE;
-#pragma unroll
+#pragma unroll 2
         for (int u0 = 0; u0 < ID::UNITS; u0 += 64 * WR) {
             const int u = u0 + tid;
             if (ID::UNITS % (64 * WR) == 0 || u < ID::UNITS) {
@@ -206,6 +249,44 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
                 *reinterpret_cast<__attribute__((address_space(3))) h8*>(dst + slot_of(2 * ch + 1, key) * 16) =
                     bytes8_to_h8<KV>((uint32_t)raw.z, (uint32_t)raw.w);
             }
+        }
+    };
+
+    // A drafted V row that is not finite must not reach the rows that do not see
+    // it (0 x inf in the matrix product): such values of block kb are replaced
+    // by 0 in LDS, and the outputs that attend them are marked, to become NaN
+    // at the end.  (Only blocks that reach into a tree; in registers and
+    // unrolled this cost the main loop 60 of them.)
+    auto scrub = [&](int kb) {
+        lds_char* vs = (BYTES ? lds + T::AREA + (kb % T::NF16) * DD::STAGE : lds + (kb % T::STAGES) * DD::STAGE) +
+                       DD::REGION * 16;
+#pragma unroll 1
+        for (int u = tid; u < DD::REGION; u += 64 * WR) {
+            const int ch = u >> 5, key = (u & 31) ^ ((ch & 1) * kSwz);
+            __attribute__((address_space(3))) uint16_t* e =
+                reinterpret_cast<__attribute__((address_space(3))) uint16_t*>(vs + u * 16);
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
+                if ((e[i] & 0x7C00u) == 0x7C00u) {
+                    e[i] = 0;
+                    marks[0] = marks[1] = 1;
+                    __hip_atomic_fetch_or(&bad_dims[8 * ch + i], 1u << key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+        }
+        __syncthreads();
+        if (marks[1]) {
+#pragma unroll 1
+            for (int i = tid; i < T::ROWS; i += 64 * WR) {
+                const int row = row0 + i, t = row / G;
+                if (row >= M) continue;
+                const uint32_t w = tree_window(
+                    p, sq, p.mask ? p.mask + (int64_t)(sq.q0 + t) * p.mask_words : nullptr, t, kb * kKBlk);
+                for (int d = 0; d < D; ++d)
+                    if (w & bad_dims[d]) bad_outs[i * T::DW + d / 32] |= 1u << (d & 31);
+            }
+            __syncthreads();
+            for (int i = 1 + tid; i < 2 + D; i += 64 * WR) marks[i] = 0;
+            __syncthreads();
         }
     };
 
@@ -227,8 +308,9 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
     const int vpar = (c >> 1) & 1;
     const int vbase = DD::REGION * 16 + (((c & 3) >> 1) * 32 + ((4 * g + (c >> 2)) ^ (vpar * kSwz))) * 16 + 8 * (c & 1);
 
-    auto compute = [&](int kb, auto masked_tag) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
+    // One body for masked and free blocks (the mask's parts behind uniform
+    // branches): two inlined forms held 50 registers more and spilled.
+    auto compute = [&](int kb, const bool masked) {
         lds_char* sb = BYTES ? lds + T::AREA + (kb % T::NF16) * DD::STAGE : lds + (kb % T::STAGES) * DD::STAGE;
         const int key0 = kb * kKBlk;
         h8 ka[2][NC32 > 0 ? NC32 : 1];
@@ -240,13 +322,6 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
                 ka[kt][cc] = *reinterpret_cast<__attribute__((address_space(3))) h8*>(sb + kbase + (128 * cc + 16 * kt) * 16);
             if constexpr (REM)
                 kr[kt] = *reinterpret_cast<__attribute__((address_space(3))) h8*>(sb + (kt ? krb1 : krb0));
-        }
-        h8 vb[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const h4 lo = read_tr(sb + vbase + 64 * t * 16);
-            const h4 hi = read_tr(sb + vbase + (64 * t + 16) * 16);
-            vb[t] = h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
         // Scales of this lane's keys 16 kt + 4 g + r.
         float ksc[2][4], vsc[2][4];
@@ -283,85 +358,69 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) vsc[kt][r] *= vinv;
         }
-        bool tile_ok[2] = {true, true};
-        if constexpr (MASKED) {
+        uint32_t win[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) win[rb] = ~0u;
+        if (masked) {
+            uint32_t pages = ~0u;  // positions on missing pages leave
             if (any_bad) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
                     const int k16 = key0 + 16 * kt;
-                    tile_ok[kt] = k16 < k_hi && table_s[k16 / p.block_size - lb0] >= 0;
+                    if (k16 < k_hi && table_s[k16 / p.block_size - lb0] < 0) pages &= kt ? 0xFFFFu : 0xFFFF0000u;
                 }
             }
-        }
-        uint32_t win[RB];
+            const bool tree = key0 + kKBlk > sq.plain;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            win[rb] = 0;
-            if constexpr (MASKED) {
-                if (node[rb] >= 0) {
-                    const uint64_t* mrow = p.mask ? p.mask + (int64_t)(sq.q0 + node[rb]) * p.mask_words : nullptr;
-                    win[rb] = tree_window(p, sq, mrow, node[rb], key0);
+            for (int rb = 0; rb < RB; ++rb) {
+                if (tree) {
+                    const int row = row0 + 16 * (RB * wave + rb) + c, node = row / G;
+                    win[rb] = row < M ? tree_window(p, sq, p.mask ? p.mask + (int64_t)(sq.q0 + node) * p.mask_words : nullptr,
+                                                    node, key0)
+                                      : 0u;
                 }
-                if (!tile_ok[0]) win[rb] &= 0xFFFF0000u;
-                if (!tile_ok[1]) win[rb] &= 0x0000FFFFu;
+                win[rb] &= pages;
             }
         }
-        // A drafted V row that is not finite must not reach the rows that do not
-        // see it (0 x inf in the matrix product): such values leave the product,
-        // and the rows that do see them get NaN where a product of the rows'
-        // visible bits and the values' flags is not zero.
-        if constexpr (MASKED && !SCALED) {
-            uint32_t any = 0;
+        f4 sc[RB][2];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const us8 e = __builtin_bit_cast(us8, vb[t]) & (uint16_t)0x7C00;
-                const i4 w = __builtin_bit_cast(i4, (us8)(e == (uint16_t)0x7C00));
-                any |= (uint32_t)(w.x | w.y | w.z | w.w);
-            }
-            if (__any(any != 0)) {
-                h8 seen[RB];
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        seen[rb][e] = (_Float16)(int)(win[rb] >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const us8 x = __builtin_bit_cast(us8, vb[t]);
-                    const us8 not_fin = (us8)((x & (uint16_t)0x7C00) == (uint16_t)0x7C00);
-                    const h8 flag = __builtin_bit_cast(h8, (us8)(not_fin & (uint16_t)0x3C00));
-                    vb[t] = __builtin_bit_cast(h8, (us8)(x & ~not_fin));
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        const f4 hit = mfma32(seen[rb], flag, f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[rb][t][r] = hit[r] > 0.f ? __builtin_nanf("") : o[rb][t][r];
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            float sc[2][4], pf[2][4];
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int cc = 0; cc < NC32; ++cc) acc = mfma32(ka[kt][cc], qa[rb][cc], acc);
                 if constexpr (REM) acc = mfma32(kr[kt], qr[rb], acc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sc[kt][r] = acc[r];
+                sc[rb][kt] = acc;
             }
+        // (V's registers after K's: both at once pass 256 at head_dim 128)
+        __builtin_amdgcn_sched_barrier(0);
+        h8 vb[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const h4 lo = read_tr(sb + vbase + 64 * t * 16);
+            const h4 hi = read_tr(sb + vbase + (64 * t + 16) * 16);
+            vb[t] = h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            float pf[2][4];
             const uint32_t w4 = win[rb] >> (4 * g);
             auto exps = [&]() {
                 float b = 0.f;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        pf[kt][r] = fmaf(sc[rb][kt][r], SCALED ? ksc[kt][r] : p.scale_log2, -m_run[rb]);
+                if (masked)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pf[e >> 2][e & 3] = seen_or_inf(pf[e >> 2][e & 3], w4, 16 * (e >> 2) + (e & 3));
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float x = fmaf(sc[kt][r], SCALED ? ksc[kt][r] : p.scale_log2, -m_run[rb]);
-                        if constexpr (MASKED) x = (w4 >> (16 * kt + r)) & 1 ? x : -__builtin_inff();
-                        pf[kt][r] = fast_exp2(x);
+                        pf[kt][r] = fast_exp2(pf[kt][r]);
                         b += pf[kt][r];
                     }
                 return b;
@@ -373,9 +432,8 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float x = sc[kt][r] * (SCALED ? ksc[kt][r] : p.scale_log2);
-                        if constexpr (MASKED) x = (w4 >> (16 * kt + r)) & 1 ? x : -__builtin_inff();
-                        ml = vmax(ml, x);
+                        float x = sc[rb][kt][r] * (SCALED ? ksc[kt][r] : p.scale_log2);
+                        ml = vmax(ml, seen_or_inf(x, w4, 16 * kt + r));
                     }
                 ml = max_over_groups(ml);
                 const bool grow = ml > m_run[rb] + kTopLog;  // uniform per row
@@ -393,14 +451,21 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
             }
             lsum[rb] += bs;
             h8 ph, pl;
+            if constexpr (SCALED) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pf[e >> 2][e & 3] *= vsc[e >> 2][e & 3];
+                if (masked)  // (the scale of a row that is not seen may be anything)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        pf[e >> 2][e & 3] = __int_as_float(__float_as_int(pf[e >> 2][e & 3]) &
+                                                           __builtin_amdgcn_sbfe((int)w4, 16 * (e >> 2) + (e & 3), 1));
+            }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float x = pf[kt][r];
                     if constexpr (SCALED) {
-                        x *= vsc[kt][r];
-                        if constexpr (MASKED) x = (w4 >> (16 * kt + r)) & 1 ? x : 0.f;
                         // Both parts come from the rounded product: fused with
                         // it, the high part may round another way than the one
                         // that the low part is the rest of.
@@ -419,7 +484,8 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
     };
 
     // Blocks in front of the tree (and on valid pages) need no mask.
-    const int free_hi = any_bad ? kb_lo : (int)max((int64_t)kb_lo, min((int64_t)kb_hi, sq.prefix / kKBlk));
+    const int free_hi = any_bad ? kb_lo : max(kb_lo, min(kb_hi, sq.plain / kKBlk));
+    const bool busy = row0 + 16 * RB * wave < M;  // (a wave past the last row only moves data)
     constexpr int S = T::STAGES;
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
@@ -452,97 +518,117 @@ __global__ __launch_bounds__(64 * WR) void tree_kernel(TreeParams p) {
             }
         }
     };
-    for (int kb = kb_lo; kb < free_hi; ++kb) {
+    for (int kb = kb_lo; kb < kb_hi; ++kb) {
         step(kb);
-        compute(kb, std::false_type{});
-    }
-    for (int kb = free_hi; kb < kb_hi; ++kb) {
-        step(kb);
-        compute(kb, std::true_type{});
+        if constexpr (!SCALED)
+            if (kb * kKBlk + kKBlk > sq.plain) scrub(kb);
+        if (busy) compute(kb, kb >= free_hi);
     }
 
     const float vmul = SCALED ? vcap : 1.f;
-    const bool split = p.parts > 1;
-    const int64_t pbase = (int64_t)part * p.rows_cap;
+    const int64_t pbase = (piece * p.num_kv_heads + kvh) * T::ROWS;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const float l = sum_over_groups(lsum[rb]);  // row c
-        const int r16 = row0 + 16 * (RB * wave + rb);
-        if (g == 0 && r16 + c < M) {
-            const int t = (r16 + c) / G;
-            const int64_t at = (int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (r16 + c - t * G);
-            if (split) p.ws_ml[pbase * p.num_heads + at] = make_float2(m_run[rb], l);
-            else if (p.lse) p.lse[at] = l == 0.f ? -__builtin_inff() : (m_run[rb] + __log2f(l)) * 0.6931471805599453f;
+        const int w16 = 16 * (RB * wave + rb);
+        if (g == 0 && row0 + w16 + c < M) {
+            const int row = row0 + w16 + c, t = row / G;
+            if (!whole) p.ws_ml[pbase + w16 + c] = make_float2(m_run[rb], l);
+            else if (p.lse)
+                p.lse[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)] = row_lse(m_run[rb], l);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = r16 + 4 * g + r;
+            const int row = row0 + w16 + 4 * g + r;
             const float lr = shfl(l, 4 * g + r);
-            const float mul = split ? vmul : lr == 0.f ? 0.f : vmul / lr;
+            const float mul = !whole ? vmul : lr == 0.f ? 0.f : vmul / lr;
             if (row < M) {
                 const int t = row / G;
-                const int64_t at = (int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G);
-                float* orow = split ? p.ws_o + (pbase * p.num_heads + at) * D : p.out + at * D;
+                float* orow = !whole ? p.ws_o + (pbase + w16 + 4 * g + r) * D
+                                     : p.out + ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D;
 #pragma unroll
                 for (int tt = 0; tt < NT; ++tt) orow[16 * tt + c] = o[rb][tt][r] * mul;
             }
         }
     }
+    if constexpr (!SCALED)
+        if (marks[0]) {
+#pragma unroll 1
+            for (int i = lane; i < 16 * RB * D; i += 64) {
+                const int w = 16 * RB * wave + i / D, d = i % D, row = row0 + w, t = row / G;
+                if (row >= M || !(bad_outs[w * T::DW + d / 32] >> (d & 31) & 1)) continue;
+                (!whole ? p.ws_o + (pbase + w) * D
+                        : p.out + ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D)[d] = __builtin_nanf("");
+            }
+        }
+    if constexpr (WR > 1) __syncthreads();  // the ring and the block ids are free for the next piece
+    }  // pieces
 }
 
-// Joins the parts of each row: thread (row, head, 4 dims).
+// Joins the pieces of each row that a range's end cut: thread (row, head, 4 dims).
+template <int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p) {
     const int s = blockIdx.x / p.max_nodes, t = blockIdx.x - s * p.max_nodes;
     const TreeSeq sq(p, s);
     if (t >= sq.n) return;
+    const TreeRanges cut(p, ROWS, threadIdx.x & 63);
+    const int64_t first = cut.first_of(p, ROWS, threadIdx.x & 63, s);
     const int D4 = p.head_dim / 4;
     const int e = blockIdx.y * 256 + threadIdx.x;
     const int h = e / D4, d = e - h * D4;
     if (h >= p.num_heads) return;
-    const int64_t at = (int64_t)(sq.q0 + t) * p.num_heads + h, step = p.rows_cap * p.num_heads;
-    const int live = max(1, (sq.end + p.part_len - 1) / p.part_len);
+    const int kvh = h / p.group, row = t * p.group + (h - kvh * p.group);
+    const int blocks = (sq.end + 31) / 32;
+    const int64_t unit0 = first + (int64_t)(row / ROWS) * blocks;
+    const int r0 = cut.range_of(unit0), r1 = cut.range_of(unit0 + blocks - 1);
+    if (r0 == r1) return;  // whole in one range
+    const int64_t head0 = (int64_t)kvh * ROWS + row % ROWS, step = (int64_t)p.num_kv_heads * ROWS;
+    const int64_t at0 = (r0 * 2 + (cut.start(r0) < unit0 ? 1 : 0)) * step + head0;
+    const auto at = [&](int r) { return r == r0 ? at0 : r * 2 * step + head0; };
     float m = kMaxSeed;
-    for (int k = 0; k < live; ++k) m = fmaxf(m, p.ws_ml[k * step + at].x);
+    for (int r = r0; r <= r1; ++r) m = fmaxf(m, p.ws_ml[at(r)].x);
     float l = 0.f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < live; ++k) {
-        const float2 ml = p.ws_ml[k * step + at];
+    for (int r = r0; r <= r1; ++r) {
+        const float2 ml = p.ws_ml[at(r)];
         const float w = fast_exp2(ml.x - m);
         l += ml.y * w;
-        o += *reinterpret_cast<const f4*>(p.ws_o + ((k * step + at) * D4 + d) * 4) * w;
+        o += *reinterpret_cast<const f4*>(p.ws_o + (at(r) * D4 + d) * 4) * w;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<f4*>(p.out + (at * D4 + d) * 4) = o * inv;
-    if (d == 0 && p.lse) p.lse[at] = l == 0.f ? -__builtin_inff() : (m + __log2f(l)) * 0.6931471805599453f;
+    const int64_t to = (int64_t)(sq.q0 + t) * p.num_heads + h;
+    *reinterpret_cast<f4*>(p.out + (to * D4 + d) * 4) = o * inv;
+    if (d == 0 && p.lse) p.lse[to] = row_lse(m, l);
 }
 
 template <int KV, int D, int RB, int WR, int ST>
 hipError_t launch_tile(const TreeParams& p, hipStream_t stream) {
     using T = TreeDims<KV, D, RB, WR, ST>;
-    const int entries = p.part_len / p.block_size + 2;
-    const size_t lds = T::TABLE + (size_t)entries * 4;
+    const size_t lds = T::TABLE + (size_t)p.table_cap * 4;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void*)tree_kernel<KV, D, RB, WR, ST>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    const int64_t cells = (int64_t)p.num_seqs * p.parts;
-    const int64_t grid = (cells + 7) / 8 * 8 * p.num_kv_heads * p.row_tiles;
+    const int64_t grid = (int64_t)(p.ranges + 7) / 8 * 8 * p.num_kv_heads;
     tree_kernel<KV, D, RB, WR, ST><<<dim3((uint32_t)grid), dim3(64 * WR), lds, stream>>>(p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.ranges == 1) return e;
+    const uint32_t chunks = (uint32_t)((p.num_heads * (p.head_dim / 4) + 255) / 256);
+    tree_merge_kernel<T::ROWS><<<dim3((uint32_t)(p.num_seqs * p.max_nodes), chunks), dim3(256), 0, stream>>>(p);
     return hipGetLastError();
 }
 
 // Tiles of a shape: RB row blocks per wave and WR waves by the rows of a tree.
 template <int KV, int D>
 hipError_t launch_shape(const TreeParams& p, hipStream_t stream) {
+    constexpr int RB = D <= 80 ? T_RB : 2;
     switch (tree_tile_rows(KV, D, p.max_nodes * p.group)) {
         case 16: return launch_tile<KV, D, 1, 1, 3>(p, stream);
         case 32: return launch_tile<KV, D, 2, 1, 3>(p, stream);
-        case 64: return D <= 80 ? launch_tile<KV, D, D <= 80 ? 4 : 2, D <= 80 ? 1 : 2, 3>(p, stream)
-                                : launch_tile<KV, D, 2, 2, 3>(p, stream);
-        case 128: return D <= 80 ? launch_tile<KV, D, D <= 80 ? 4 : 2, D <= 80 ? 2 : 4, 4>(p, stream)
-                                 : launch_tile<KV, D, 2, 4, 4>(p, stream);
-        default: return launch_tile<KV, D, D <= 80 ? 4 : 2, 4, 4>(p, stream);
+        case 64: return launch_tile<KV, D, RB, 4 / RB, 3>(p, stream);
+        case 128: return launch_tile<KV, D, RB, 8 / RB, T_ST>(p, stream);
+        default: return launch_tile<KV, D, RB, 4, T_ST>(p, stream);
     }
 }
 
@@ -559,7 +645,7 @@ hipError_t launch_dim(const TreeParams& p, hipStream_t stream) {
 }  // namespace
 
 int tree_tile_rows(int kv_dtype, int head_dim, int rows) {
-    const int most = head_dim <= 80 ? 256 : 128;
+    const int most = 64 * (head_dim <= 80 ? T_RB : 2);
     for (int t = 16; t < most; t *= 2)
         if (rows <= t) return t;
     return most;
@@ -571,17 +657,12 @@ int tree_wgs_per_cu(int kv_dtype, int head_dim, int rows) {
 }
 
 hipError_t launch_tree(const TreeParams& p, hipStream_t stream) {
-    hipError_t e;
     switch (p.kv_dtype) {
-        case VCPP_KV_F16: e = launch_dim<VCPP_KV_F16>(p, stream); break;
-        case VCPP_KV_I8: e = launch_dim<VCPP_KV_I8>(p, stream); break;
-        case VCPP_KV_FP8: e = launch_dim<VCPP_KV_FP8>(p, stream); break;
+        case VCPP_KV_F16: return launch_dim<VCPP_KV_F16>(p, stream);
+        case VCPP_KV_I8: return launch_dim<VCPP_KV_I8>(p, stream);
+        case VCPP_KV_FP8: return launch_dim<VCPP_KV_FP8>(p, stream);
         default: return hipErrorInvalidValue;
     }
-    if (e != hipSuccess || p.parts <= 1) return e;
-    const uint32_t chunks = (uint32_t)((p.num_heads * (p.head_dim / 4) + 255) / 256);
-    tree_merge_kernel<<<dim3((uint32_t)(p.num_seqs * p.max_nodes), chunks), dim3(256), 0, stream>>>(p);
-    return hipGetLastError();
 }
 
 }  // namespace vcpp
