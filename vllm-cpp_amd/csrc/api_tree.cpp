@@ -49,8 +49,8 @@ struct TreeSplit {
 
 // Ranges: one per workgroup (and kv head) that the GPU holds at once, fewer
 // where the bounds allow fewer than kTreeMinBlocks blocks each, more where a
-// range's block ids would pass kMaxTable.
-constexpr int64_t kMaxTable = 2048;
+// range's tile table in LDS would pass kMaxRange blocks (8 or 16 KB).
+constexpr int64_t kMaxRange = 512;
 
 TreeSplit tree_split(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t max_nodes, int32_t max_prefix_len,
                      int32_t num_heads) {
@@ -62,11 +62,10 @@ TreeSplit tree_split(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t max_node
     const int64_t slots = (int64_t)vcpp::compute_units() * vcpp::tree_wgs_per_cu(kv->dtype, kv->head_dim, rows);
     int64_t R = std::min(std::max<int64_t>(1, slots / kv->num_kv_heads), std::max<int64_t>(1, most / vcpp::kTreeMinBlocks));
     // (a piece is no longer than its sequence, nor than its range)
-    const int64_t per_range = kMaxTable * kv->block_size / 32 - 4;
-    if (blocks > per_range) R = std::max(R, (most + per_range - 1) / per_range);
+    if (blocks > kMaxRange - 4) R = std::max(R, (most + kMaxRange - 5) / (kMaxRange - 4));
     t.ranges = (int32_t)std::min<int64_t>(R, INT32_MAX);
     const int64_t longest = std::min(blocks, std::max<int64_t>((most + R - 1) / R, 2 * vcpp::kTreeMinBlocks) + 1);
-    t.table_cap = (int32_t)(longest * 32 / kv->block_size + 2);
+    t.table_cap = (int32_t)(2 * longest);
     if (t.ranges > 1) {
         const size_t n = (size_t)t.ranges * 2 * kv->num_kv_heads * tile;
         t.off_ml = align256(n * kv->head_dim * sizeof(float));

@@ -47,7 +47,7 @@ struct TreeParams {
     // Key split (attention): the units (sequence, row tile), each as long as its
     // key blocks, are cut into `ranges` equal ranges (TreeRanges).
     int32_t ranges;
-    int32_t table_cap; // block ids of a range's longest piece
+    int32_t table_cap; // 16-position tiles of a range's longest piece
     int64_t rows_cap;  // num_seqs * max_nodes
     float* ws_o;       // [ranges][2][num_kv_heads][tile rows][head_dim]
     float2* ws_ml;     // [ranges][2][num_kv_heads][tile rows] (exponent in log2 units, sum)

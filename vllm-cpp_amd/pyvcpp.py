@@ -304,33 +304,32 @@ def paged_prefill_split(pages, q, out, block_tables, q_start, prefix_lens, max_c
     return out
 
 
-def _operand(name, t, dtype, shape=None):
-    """Address of a dense tensor of this dtype (and shape) on the current
-    device; anything else would be misread."""
-    import torch
-    if t.dtype is not dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError("%s must be a contiguous %s tensor%s, got %s %s with strides %s" % (
-            name, dtype, " of shape %s" % (shape,) if shape else "", t.dtype, tuple(t.shape), t.stride()))
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError("%s is on %s, not on the current GPU" % (name, t.device))
-    return t.data_ptr()
+class _Operands:
+    """Checks a call's tensors -- dense, of the right type and shape, on the
+    current GPU; anything else would be misread -- and gives their addresses."""
+
+    def __init__(self):
+        import torch
+        self.device = torch.cuda.current_device()
+        self.f16, self.f32, self.i32, self.i64 = torch.float16, torch.float32, torch.int32, torch.int64
+
+    def __call__(self, name, t, dtype, shape=None):
+        if t is None:
+            return None
+        if t.dtype is not dtype or (shape is not None and t.shape != shape) or not t.is_contiguous():
+            raise ValueError("%s must be a contiguous %s tensor%s, got %s %s with strides %s" % (
+                name, dtype, "" if shape is None else " of shape %s" % (tuple(shape),), t.dtype, tuple(t.shape), t.stride()))
+        if t.get_device() != self.device:
+            raise ValueError("%s is on %s, not on the current GPU" % (name, t.device))
+        return t.data_ptr()
+
+    def stream(self, stream):
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else stream.cuda_stream
 
 
 def tree_workspace_size(pages, num_seqs, max_nodes, max_prefix_len, num_heads):
     return lib().vcpp_tree_workspace_size(ctypes.byref(pages), num_seqs, max_nodes, max_prefix_len, num_heads)
-
-
-def _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens, tree_mask, num_heads):
-    """Checked addresses of what the tree calls share."""
-    import torch
-    rows, S = q.shape[0], prefix_lens.shape[0]
-    words = 0 if tree_mask is None else tree_mask.shape[-1]
-    mask = None if tree_mask is None else _operand("tree_mask", tree_mask, torch.int64, (rows, words))
-    z = None if lse is None else _operand("lse", lse, torch.float32, (rows, num_heads))
-    return (_operand("q", q, torch.float16, (rows, num_heads, pages.head_dim)), z,
-            _operand("block_tables", block_tables, torch.int32, (S, block_tables.shape[-1])), block_tables.shape[-1],
-            _operand("q_start", q_start, torch.int32, (S + 1,)), _operand("prefix_lens", prefix_lens, torch.int32, (S,)),
-            mask, words, S)
 
 
 def paged_tree_attention(pages, q, out, block_tables, q_start, prefix_lens, max_nodes, max_prefix_len, num_heads,
@@ -338,33 +337,41 @@ def paged_tree_attention(pages, q, out, block_tables, q_start, prefix_lens, max_
     """vcpp_paged_tree_attention: q fp16 [rows][H][D], out fp32 [rows][H][D],
     lse fp32 [rows][H] or None, tree_mask int64 [rows][words] (the words' bits)
     or None for chains."""
-    import torch
-    qp, lp, bt, mb, st, pf, mask, words, S = _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens,
-                                                            tree_mask, num_heads)
-    o = _operand("out", out, torch.float32, tuple(q.shape))
-    if q.shape[0] > S * max_nodes:
-        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (q.shape[0], S, max_nodes))
+    op = _Operands()
+    shape, S = q.shape, prefix_lens.shape[0]
+    rows, blocks = shape[0], block_tables.shape[-1]
+    words = 0 if tree_mask is None else tree_mask.shape[-1]
+    if rows > S * max_nodes:
+        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (rows, S, max_nodes))
     if workspace is None:
+        import torch
         need = tree_workspace_size(pages, S, max_nodes, max_prefix_len, num_heads)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    ws, nbytes = (None, 0) if workspace is None else (_operand("workspace", workspace, torch.uint8), workspace.numel())
-    _check(lib().vcpp_paged_tree_attention(ctypes.byref(pages), qp, o, lp, bt, mb, st, pf, mask, words, S, max_nodes,
-                                           max_prefix_len, num_heads, ws, nbytes, _stream(stream)))
+    _check(lib().vcpp_paged_tree_attention(
+        ctypes.byref(pages), op("q", q, op.f16, (rows, num_heads, pages.head_dim)), op("out", out, op.f32, shape),
+        op("lse", lse, op.f32, (rows, num_heads)), op("block_tables", block_tables, op.i32, (S, blocks)), blocks,
+        op("q_start", q_start, op.i32, (S + 1,)), op("prefix_lens", prefix_lens, op.i32, (S,)),
+        op("tree_mask", tree_mask, op.i64, (rows, words)), words, S, max_nodes, max_prefix_len, num_heads,
+        None if workspace is None else op("workspace", workspace, workspace.dtype),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), op.stream(stream)))
     return out
 
 
 def attention_mass(pages, q, lse, scores, block_tables, q_start, prefix_lens, max_nodes, max_prefix_len, num_heads,
                    tree_mask=None, stream=None):
     """vcpp_attention_mass: adds to scores fp32 [S][Hkv][stride] in place."""
-    import torch
-    qp, lp, bt, mb, st, pf, mask, words, S = _tree_operands(pages, q, lse, block_tables, q_start, prefix_lens,
-                                                            tree_mask, num_heads)
-    if q.shape[0] > S * max_nodes:
-        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (q.shape[0], S, max_nodes))
-    stride = scores.shape[-1]
-    sc = _operand("scores", scores, torch.float32, (S, pages.num_kv_heads, stride))
-    _check(lib().vcpp_attention_mass(ctypes.byref(pages), qp, lp, sc, stride, bt, mb, st, pf, mask, words, S, max_nodes,
-                                     max_prefix_len, num_heads, _stream(stream)))
+    op = _Operands()
+    rows, S, stride = q.shape[0], prefix_lens.shape[0], scores.shape[-1]
+    blocks = block_tables.shape[-1]
+    words = 0 if tree_mask is None else tree_mask.shape[-1]
+    if rows > S * max_nodes:
+        raise ValueError("%d rows are more than %d sequences of %d nodes hold" % (rows, S, max_nodes))
+    _check(lib().vcpp_attention_mass(
+        ctypes.byref(pages), op("q", q, op.f16, (rows, num_heads, pages.head_dim)), op("lse", lse, op.f32, (rows, num_heads)),
+        op("scores", scores, op.f32, (S, pages.num_kv_heads, stride)), stride,
+        op("block_tables", block_tables, op.i32, (S, blocks)), blocks, op("q_start", q_start, op.i32, (S + 1,)),
+        op("prefix_lens", prefix_lens, op.i32, (S,)), op("tree_mask", tree_mask, op.i64, (rows, words)), words, S,
+        max_nodes, max_prefix_len, num_heads, op.stream(stream)))
     return scores
 
 
@@ -373,41 +380,38 @@ def kv_evict_plan(scores, context_lens, max_context_len, budget, moves, move_cou
     """vcpp_kv_evict_plan: scores fp32 [S][Hkv][stride] (and positions int32)
     to moves int32 [S][Hkv][n][2], move_counts [S][Hkv], new_lens [S] and the
     state after the moves."""
-    import torch
-    S, hkv, stride = scores.shape
-    i32, shape = torch.int32, (S, hkv, stride)
+    op = _Operands()
+    shape = scores.shape
+    S, hkv, stride = shape
+    n = moves.shape[2]
     _check(lib().vcpp_kv_evict_plan(
-        _operand("scores", scores, torch.float32), None if positions is None else _operand("positions", positions, i32, shape),
-        stride, _operand("context_lens", context_lens, i32, (S,)),
-        None if seen_lens is None else _operand("seen_lens", seen_lens, i32, (S,)), S, hkv, max_context_len, budget,
-        keep_first, keep_last, _operand("moves", moves, i32, (S, hkv, moves.shape[2], 2)), moves.shape[2],
-        _operand("move_counts", move_counts, i32, (S, hkv)), _operand("new_lens", new_lens, i32, (S,)),
-        _operand("scores_out", scores_out, torch.float32, shape),
-        None if positions_out is None else _operand("positions_out", positions_out, i32, shape), _stream(stream)))
+        op("scores", scores, op.f32), op("positions", positions, op.i32, shape), stride,
+        op("context_lens", context_lens, op.i32, (S,)), op("seen_lens", seen_lens, op.i32, (S,)), S, hkv, max_context_len,
+        budget, keep_first, keep_last, op("moves", moves, op.i32, (S, hkv, n, 2)), n,
+        op("move_counts", move_counts, op.i32, (S, hkv)), op("new_lens", new_lens, op.i32, (S,)),
+        op("scores_out", scores_out, op.f32, shape), op("positions_out", positions_out, op.i32, shape), op.stream(stream)))
 
 
 def kv_evict_apply(pages, block_tables, moves, move_counts, stream=None):
     """vcpp_kv_evict_apply: the planned row moves inside the pages."""
-    import torch
+    op = _Operands()
     S, blocks = block_tables.shape
-    n = moves.shape[2]
+    hkv, n = pages.num_kv_heads, moves.shape[2]
     _check(lib().vcpp_kv_evict_apply(
-        ctypes.byref(pages), _operand("block_tables", block_tables, torch.int32), blocks,
-        _operand("moves", moves, torch.int32, (S, pages.num_kv_heads, n, 2)), n,
-        _operand("move_counts", move_counts, torch.int32, (S, pages.num_kv_heads)), S, _stream(stream)))
+        ctypes.byref(pages), op("block_tables", block_tables, op.i32), blocks, op("moves", moves, op.i32, (S, hkv, n, 2)), n,
+        op("move_counts", move_counts, op.i32, (S, hkv)), S, op.stream(stream)))
 
 
 def kv_commit(pages, block_tables, prefix_lens, accepted, accept_lens, max_nodes, num_layers=1, layer_stride=0,
               scale_layer_stride=0, stream=None):
     """vcpp_kv_commit: accepted int32 [S][n] node indices, accept_lens int32 [S]."""
-    import torch
+    op = _Operands()
     S, blocks = block_tables.shape
     n = accepted.shape[1]
     _check(lib().vcpp_kv_commit(
-        ctypes.byref(pages), _operand("block_tables", block_tables, torch.int32), blocks,
-        _operand("prefix_lens", prefix_lens, torch.int32, (S,)), _operand("accepted", accepted, torch.int32, (S, n)),
-        _operand("accept_lens", accept_lens, torch.int32, (S,)), S, n, max_nodes, num_layers, layer_stride,
-        scale_layer_stride, _stream(stream)))
+        ctypes.byref(pages), op("block_tables", block_tables, op.i32), blocks, op("prefix_lens", prefix_lens, op.i32, (S,)),
+        op("accepted", accepted, op.i32, (S, n)), op("accept_lens", accept_lens, op.i32, (S,)), S, n, max_nodes, num_layers,
+        layer_stride, scale_layer_stride, op.stream(stream)))
 
 
 def write_kv(pages, k, v, slots, fp16_round_nearest=False, stream=None):
