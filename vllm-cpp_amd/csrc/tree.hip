@@ -22,8 +22,8 @@
 // (P <= 2^15), so that the low part of a P of 2^-16 of the row's largest still
 // has 19 bits; it moves when a row's largest score grows by more than 2^4.
 // int8 pages: K and V are exact fp16 integers; the key's K scale multiplies
-// the score, its V scale P (over a running power of two, so that any scale
-// keeps P in fp16's range).
+// the score, its V scale P (whose exponent is lowered by a running power of two
+// at or above the scales, so that any scale keeps the product in range).
 #include "prefill_body.h"
 #include "profile.h"
 #include "tree.h"
@@ -99,7 +99,8 @@ struct TreeDims {
     // Windows (tree_window) of the tile's rows on the key blocks that reach into
     // a tree: at most 9.
     static constexpr int WINDOWS = MARKS + (SCALED ? 0 : (2 + D + ROWS * DW) * 4);
-    static constexpr int TABLE = (WINDOWS + (kMaxTreeNodes / kKBlk + 1) * ROWS * 4 + 7) & ~7;
+    static constexpr int SEQS = WINDOWS + (kMaxTreeNodes / kKBlk + 1) * ROWS * 4;  // the (at most 64) sequences
+    static constexpr int TABLE = (SEQS + kWave * (int)sizeof(TreeSeq) + 7) & ~7;
     static_assert(STAGES >= 3 && (STAGES - 1) * PERW < 64, "ring depth");
 };
 
@@ -173,15 +174,33 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
     const int jj = blockIdx.x >> 3;
     const int kvh = jj % p.num_kv_heads;
     const int range = (jj / p.num_kv_heads) * 8 + (blockIdx.x & 7);
-    const TreeRanges cut(p, T::ROWS, lane);
+    TreeRanges cut(p, T::ROWS, lane);
     if (range >= cut.R || cut.total == 0) return;  // whole workgroup
     const int64_t lo = cut.start(range), hi = cut.start(range + 1);
     int64_t first;  // first block of sequence s
-    int s = cut.seq_of(p, T::ROWS, lane, lo, first);
+    int s = cut.seq_of(lo, first);
+    // (in LDS: in the lanes they would hold registers through the loop)
+    __attribute__((address_space(3))) int32_t* seqs =
+        reinterpret_cast<__attribute__((address_space(3))) int32_t*>(lds + T::SEQS);
+    if (p.num_seqs <= kWave && wave == 0) {
+        const int v[5] = {cut.mine.q0, cut.mine.n, cut.mine.prefix, cut.mine.end, cut.mine.plain};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) seqs[5 * lane + i] = v[i];
+    }
+    __syncthreads();
     const int G = p.group;
     int64_t at_block = lo;
     while (at_block < hi) {  // the range's pieces, one per unit
-    const TreeSeq sq(p, s);
+    TreeSeq sq;
+    if (p.num_seqs <= kWave) {
+        sq.q0 = __builtin_amdgcn_readfirstlane(seqs[5 * s]);
+        sq.n = __builtin_amdgcn_readfirstlane(seqs[5 * s + 1]);
+        sq.prefix = __builtin_amdgcn_readfirstlane(seqs[5 * s + 2]);
+        sq.end = __builtin_amdgcn_readfirstlane(seqs[5 * s + 3]);
+        sq.plain = __builtin_amdgcn_readfirstlane(seqs[5 * s + 4]);
+    } else {
+        sq = TreeSeq(p, s);
+    }
     const int M = sq.n * G;
     const int tiles = (M + T::ROWS - 1) / T::ROWS, blocks = (sq.end + 31) / 32;
     if (at_block >= first + (int64_t)tiles * blocks) {  // next sequence
@@ -189,7 +208,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
         ++s;
         continue;
     }
-    const int rt = (int)((at_block - first) / blocks);
+    const int rt = (int)((uint32_t)(at_block - first) / (uint32_t)blocks);  // (a sequence's blocks: below 2^31)
     const int64_t unit0 = first + (int64_t)rt * blocks;  // the unit's first block
     const int kb_lo = (int)(at_block - unit0);
     const int kb_hi = (int)min((int64_t)blocks, hi - unit0);
@@ -199,12 +218,13 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
     const int row0 = rt * T::ROWS;
     const int k_lo = kb_lo * kKBlk, k_hi = min(kb_hi * kKBlk, sq.end);
 
-    // Q fragments (B operand): row row0 + 16 (RB wave + rb) + c
+    // Q fragments (B operand): row row0 + 16 (WR rb + wave) + c (a tile that is
+    // not full keeps every wave busy)
     h8 qa[RB][NC32 > 0 ? NC32 : 1];
     h8 qr[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int row = row0 + 16 * (RB * wave + rb) + c;
+        const int row = row0 + 16 * (WR * rb + wave) + c;
         const bool ok = row < M;
         const int t = ok ? row / G : 0;
         const _Float16* qrow = reinterpret_cast<const _Float16*>(p.q) +
@@ -305,19 +325,24 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
             }
         }
         lds_char* dst0 = lds + T::AREA + (kb % T::NF16) * DD::STAGE;
+        const auto unit = [&](int u, lds_char* dst, int slot) {  // raw unit u to slots `slot` and the row's next chunk
+            const i4 raw = *reinterpret_cast<__attribute__((address_space(3))) i4*>(st + u * 16);
+            *reinterpret_cast<__attribute__((address_space(3))) h8*>(dst + slot * 16) =
+                bytes8_to_h8<KV>((uint32_t)raw.x, (uint32_t)raw.y);
+            *reinterpret_cast<__attribute__((address_space(3))) h8*>(dst + (is_pow2(DD::NCH) ? slot ^ 1 : slot + 1) * 16) =
+                bytes8_to_h8<KV>((uint32_t)raw.z, (uint32_t)raw.w);
+        };
+        if constexpr (ID::REGION % (64 * WR) == 0) {  // a thread's units are 64 WR / NCH keys apart, K's then V's
+            constexpr int EACH = ID::REGION / (64 * WR), STEP = 64 * WR / ID::NCH;
+            const int slot = slot_at<DD::NCH>(tid / ID::NCH, 2 * (tid % ID::NCH));
+#pragma unroll
+            for (int i = 0; i < 2 * EACH; ++i)
+                unit(tid + 64 * WR * i, dst0 + (i / EACH * DD::REGION + i % EACH * STEP * DD::NCH) * 16, slot);
+        } else {
 #pragma unroll 1
-        for (int u0 = 0; u0 < ID::UNITS; u0 += 64 * WR) {
-            const int u = u0 + tid;
-            if (ID::UNITS % (64 * WR) == 0 || u < ID::UNITS) {
-                const int which = u >= ID::REGION;
-                const int q = u - which * ID::REGION;
-                const int key = q / ID::NCH, ch = q % ID::NCH;
-                const i4 raw = *reinterpret_cast<__attribute__((address_space(3))) i4*>(st + u * 16);
-                lds_char* dst = dst0 + which * DD::REGION * 16;
-                *reinterpret_cast<__attribute__((address_space(3))) h8*>(dst + slot_at<DD::NCH>(key, 2 * ch) * 16) =
-                    bytes8_to_h8<KV>((uint32_t)raw.x, (uint32_t)raw.y);
-                *reinterpret_cast<__attribute__((address_space(3))) h8*>(dst + slot_at<DD::NCH>(key, 2 * ch + 1) * 16) =
-                    bytes8_to_h8<KV>((uint32_t)raw.z, (uint32_t)raw.w);
+            for (int u = tid; u < ID::UNITS; u += 64 * WR) {
+                const int which = u >= ID::REGION, q = u - which * ID::REGION;
+                unit(u, dst0 + which * DD::REGION * 16, slot_at<DD::NCH>(q / ID::NCH, 2 * (q % ID::NCH)));
             }
         }
     };
@@ -365,7 +390,9 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
         lsum[rb] = 0.f;
         m_run[rb] = kMaxSeed;
     }
-    float vcap = 0.f, vinv = 0.f;  // int8: power of two at or above every finite V scale so far, and its inverse
+    // int8: a power of two 2^vexp at or above every finite V scale so far
+    // divides P (it is part of m_run), so that P times a scale stays in range.
+    float vcap = 0x1p-24f, vexp = -24.f, p_top = SCALED ? kTopP * 0x1p24f : kTopP;
 
     // LDS byte offsets of this lane's fragment reads.  K: row 16 kt + c, chunks
     // 4 cc + g; V: rows 16 hh + 4 g + c / 4, half c & 1 of chunk 2 t + (c & 3) / 2.
@@ -380,6 +407,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
     for (int i = 0; i < NV; ++i)
         vat[i] = DD::REGION * 16 + slot_at<DD::NCH>(4 * g + (c >> 2), 2 * i + ((c & 3) >> 1)) * 16 + 8 * (c & 1);
 
+    const int live = (M - row0 - 16 * wave + 16 * WR - 1) / (16 * WR);  // this wave's row blocks that hold rows (<= 0: none)
     // One key block (K and V at `at`) for this wave's rows, SG row blocks at a
     // time.  One body for masked and free blocks (the mask's parts behind
     // uniform branches): two inlined forms held 50 registers more and spilled.
@@ -409,18 +437,23 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(b[r]) < 65536.f ? fabsf(b[r]) : 0.f);  // (finite ones)
             }
-            if (__any(top > vcap)) {
+            if (__builtin_expect(__any(top > vcap), 0)) {
+                asm volatile("" : "+v"(top));  // (a branch: as selects its products run for every block)
                 top = fmaxf(top, shfl_xor(top, 16));
                 top = fmaxf(top, shfl_xor(top, 32));
                 const uint32_t up = (__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u;  // (fp16 scales are normal in fp32)
                 const float cap = fmaxf(__uint_as_float(up), vcap);
-                const float down = vcap / cap;
+                const float down = vcap / cap, by = (float)((int)(__float_as_uint(cap) >> 23) - 127) - vexp;
                 vcap = cap;
-                vinv = 1.f / cap;
+                vexp += by;
+                p_top = kTopP / cap;
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
+                for (int rb = 0; rb < RB; ++rb) {
+                    m_run[rb] += by;
+                    lsum[rb] *= down;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) o[rb][t] *= down;
+                }
             }
         }
         // Bits 16 kt + r: key 16 kt + 4 g + r is seen by row c of row block rb.
@@ -431,13 +464,14 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
                 for (int kt = 0; kt < 2; ++kt)
                     if (table_s[2 * (kb - kb_lo) + kt] < 0) w &= kt ? 0xFFFFu : 0xFFFF0000u;
             }
-            if (kb >= tree_kb) w &= windows[(kb - tree_kb) * T::ROWS + 16 * (RB * wave + rb) + c];
+            if (kb >= tree_kb) w &= windows[(kb - tree_kb) * T::ROWS + 16 * (WR * rb + wave) + c];
             return w >> (4 * g);
         };
-        constexpr int SG = RB == 2 ? 2 : 1;
+        constexpr int SG = 1;
         h8 vb[NT];
 #pragma unroll
         for (int r0 = 0; r0 < RB; r0 += SG) {
+            if (r0 >= live) break;
             f4 sc[SG][2];
 #pragma unroll
             for (int i = 0; i < SG; ++i)
@@ -485,7 +519,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
 #pragma unroll
             for (int i = 0; i < SG; ++i) {
                 exps(i);
-                cross |= !(bs[i] <= kTopP);
+                cross |= !(bs[i] <= p_top);
             }
             if (__builtin_expect(__any(cross), 0)) {
 #pragma unroll
@@ -501,6 +535,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
                         for (int r = 0; r < 4; ++r) ml = vmax(ml, seen_or_inf(sc[i][kt][r] * ks[r], w, 16 * kt + r));
                     }
                     ml = max_over_groups(ml);
+                    if constexpr (SCALED) ml += vexp;
                     const bool grow = ml > m_run[rb] + kTopLog;  // uniform per row
                     const float m_new = grow ? ml - kHead : m_run[rb];
                     const float alpha = fast_exp2(m_run[rb] - m_new);
@@ -525,7 +560,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
                     for (int kt = 0; kt < 2; ++kt) {
                         const f4 vs = scale4(kt, true);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) pf[i][4 * kt + r] *= vs[r] * vinv;
+                        for (int r = 0; r < 4; ++r) pf[i][4 * kt + r] *= vs[r];
                     }
                     if (masked) {  // (the scale of a row that is not seen may be anything)
                         uint32_t w = seen(rb);
@@ -548,7 +583,6 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
 
     // Blocks in front of the tree (and on valid pages) need no mask.
     const int free_hi = any_bad ? kb_lo : max(kb_lo, min(kb_hi, tree_kb));
-    const bool busy = row0 + 16 * RB * wave < M;  // (a wave past the last row only moves data)
     constexpr int S = T::STAGES;
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
@@ -584,17 +618,16 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
         }
         if constexpr (!SCALED)
             if (kb >= tree_kb) scrub(kb);
-        if (busy)
+        if (live > 0)
             compute(kb, kb >= free_hi, BYTES ? lds + T::AREA + (kb % T::NF16) * DD::STAGE : lds + rd_at);
         rd_at = next(rd_at);
     }
 
-    const float vmul = SCALED ? vcap : 1.f;
     const int64_t pbase = (piece * p.num_kv_heads + kvh) * T::ROWS;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const float l = sum_over_groups(lsum[rb]);  // row c
-        const int w16 = 16 * (RB * wave + rb);
+        const int w16 = 16 * (WR * rb + wave);
         if (g == 0 && row0 + w16 + c < M) {
             const int row = row0 + w16 + c, t = row / G;
             if (!whole) p.ws_ml[pbase + w16 + c] = make_float2(m_run[rb], l);
@@ -605,7 +638,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
         for (int r = 0; r < 4; ++r) {
             const int row = row0 + w16 + 4 * g + r;
             const float lr = shfl(l, 4 * g + r);
-            const float mul = !whole ? vmul : lr == 0.f ? 0.f : vmul / lr;
+            const float mul = !whole ? 1.f : lr == 0.f ? 0.f : 1.f / lr;
             if (row < M) {
                 const int t = row / G;
                 float* orow = !whole ? p.ws_o + (pbase + w16 + 4 * g + r) * D
@@ -619,7 +652,7 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
         if (marks[0]) {
 #pragma unroll 1
             for (int i = lane; i < 16 * RB * D; i += 64) {
-                const int w = 16 * RB * wave + i / D, d = i % D, row = row0 + w, t = row / G;
+                const int w = 16 * (WR * (i / (16 * D)) + wave) + i / D % 16, d = i % D, row = row0 + w, t = row / G;
                 if (row >= M || !(bad_outs[w * T::DW + d / 32] >> (d & 31) & 1)) continue;
                 (!whole ? p.ws_o + (pbase + w) * D
                         : p.out + ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D)[d] = __builtin_nanf("");
@@ -654,8 +687,8 @@ __global__ __launch_bounds__(256) void tree_merge_few_kernel(TreeParams p) {
     const int s = blockIdx.x / p.max_nodes, t = blockIdx.x - s * p.max_nodes;
     const TreeSeq sq(p, s);
     if (t >= sq.n) return;
-    const TreeRanges cut(p, ROWS, threadIdx.x & 63);
-    const int64_t first = cut.first_of(p, ROWS, threadIdx.x & 63, s);
+    TreeRanges cut(p, ROWS, threadIdx.x & 63);
+    const int64_t first = cut.first_of(s);
     const int e = blockIdx.y * 256 + threadIdx.x;
     const int h = e / D4, d = e - h * D4;
     if (h >= p.num_heads) return;
@@ -706,8 +739,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeParams p, int heads
     const int lane = threadIdx.x & 63;
     const TreeSeq sq(p, s);
     if (t >= sq.n) return;
-    const TreeRanges cut(p, ROWS, lane);
-    const int64_t first = cut.first_of(p, ROWS, lane, s);
+    TreeRanges cut(p, ROWS, lane);
+    const int64_t first = cut.first_of(s);
     const int blocks = (sq.end + 31) / 32;
     const int d = lane % D4, sl = lane / D4;
     const int h0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * heads;
