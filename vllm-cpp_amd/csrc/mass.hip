@@ -9,7 +9,8 @@
 // rows along a lane's accumulators, so that a lane sums its position's weights
 // in registers and only the four lane groups meet at the end.  K goes straight
 // from its pages to the product's operands (a lane's 16 bytes are 16 bytes of
-// its position's row): each row of K is read once per kv head.
+// its position's row): each row of K is read once per kv head.  The rows'
+// operands and log-sum-exps are staged in LDS, 128 rows at a time.
 #include "device_common.h"
 #include "tree.h"
 #include "tree_mask.h"
@@ -58,10 +59,19 @@ __device__ __forceinline__ void load_k(const TreeParams& p, int64_t row, int g, 
     }
 }
 
-template <int KV, int D>
+// Rows (node, head of the group) held in LDS at a time.
+constexpr int kMassRows = 128;
+
+// ONE: at most 16 rows (a decode step): their operand stays in registers, and
+// the next positions' block ids and scores are loaded beside this one's K.
+template <int KV, int D, bool ONE>
 __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
     using MD = MassDims<KV, D>;
     constexpr bool SCALED = KV == VCPP_KV_I8;
+    constexpr int RBS = ONE ? 1 : kMassRows / 16;
+    __shared__ __attribute__((aligned(16))) h8 q_s[RBS][MD::NS][kWave];     // operands as the lanes hold them
+    __shared__ __attribute__((aligned(16))) float shift_s[RBS * 16];        // log-sum-exps in log2 units
+    __shared__ uint64_t win_s[kMassWaves][RBS * 16];                        // windows of each wave's 64 positions
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     // The kv heads of one (sequence, part) share an XCD (and its L2's lines).
@@ -72,86 +82,144 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
     if (part >= p.parts) return;
     const TreeSeq sq(p, s);
     const int G = p.group, M = sq.n * G;
-    const int k_hi = min(part * p.part_len + p.part_len, sq.end);
-    if (M == 0) return;
+    const int k_lo = part * p.part_len, k_hi = min(k_lo + p.part_len, sq.end);
+    if (M == 0 || k_lo >= k_hi) return;  // whole workgroup
     const int32_t* table = p.block_tables + (int64_t)s * p.max_blocks;
     float* out = p.scores + ((int64_t)s * p.num_kv_heads + kvh) * p.score_stride;
 
-    for (int k0 = part * p.part_len + kMassKeys * wave; k0 < k_hi; k0 += kMassKeys * kMassWaves) {
+    // Rows r0 .. r0 + 16 RBS - 1 into LDS.
+    auto stage = [&](int r0) {
+        const int rows = min(M - r0, 16 * RBS), units = (rows + 15) / 16 * MD::NS * kWave;
+        for (int u = threadIdx.x; u < units; u += 64 * kMassWaves) {
+            const int l = u & 63, i = u / kWave % MD::NS, rb = u / (kWave * MD::NS);
+            const int row = r0 + 16 * rb + (l & 15), gg = l >> 4, t = row / G;
+            const bool in = row < M && (i < MD::NC || gg < 2);
+            q_s[rb][i][l] = in ? *reinterpret_cast<const h8*>(
+                                     reinterpret_cast<const _Float16*>(p.q) +
+                                     ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D + MD::dim(i, gg))
+                               : h8{};
+        }
+        for (int i = threadIdx.x; i < (rows + 15) / 16 * 16; i += 64 * kMassWaves) {
+            const int row = r0 + i, t = row / G;
+            float z = __builtin_inff();  // (rows past the last, and rows that saw nothing, add exp2(-inf))
+            if (row < M) {
+                const float x = p.lse_in[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)];
+                if (x != -__builtin_inff()) z = x * kLog2e;
+            }
+            shift_s[i] = z;
+        }
+        __syncthreads();
+    };
+    // This lane's position of the wave's 64 at k0: its block id (-1: none).
+    auto block_of = [&](int k0, int& slot) {
+        const int pos = k0 + lane;
+        const int lb = (int)(((uint64_t)(uint32_t)pos * p.bs_magic) >> 40);
+        slot = pos - lb * p.block_size;
+        const int bid = pos < k_hi && lb < p.max_blocks ? table[lb] : -1;
+        return bid >= 0 && (int64_t)bid < p.num_blocks ? bid : -1;
+    };
+    const bool several = !ONE && M > 16 * RBS;
+    constexpr int STEP = kMassKeys * kMassWaves;
+    int slot = 0, bid = block_of(k_lo + kMassKeys * wave, slot);
+    if (!several) stage(0);
+    h8 q1[MD::NS];
+    f4 shift1 = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (ONE) {
+#pragma unroll
+        for (int i = 0; i < MD::NS; ++i) q1[i] = q_s[0][i][lane];
+        shift1 = *reinterpret_cast<const f4*>(&shift_s[4 * g]);
+    }
+    for (int base = k_lo; base < k_hi; base += STEP) {  // (whole workgroup)
+        const int k0 = base + kMassKeys * wave;
+        const bool have = bid >= 0;
         h8 k[kMassTiles][MD::NS];
         float ksc[kMassTiles];
-        bool ok[kMassTiles];
+        const int64_t my_row = (int64_t)bid * p.block_stride + ((int64_t)slot * p.num_kv_heads + kvh) * D;
+        float my_scale = 0.f;
+        if constexpr (SCALED)
+            if (have)
+                my_scale = (float)__builtin_bit_cast(
+                    _Float16, p.k_scale[(int64_t)bid * p.scale_block_stride + (int64_t)kvh * p.block_size + slot]);
+        const float before = have ? out[k0 + lane] : 0.f;
 #pragma unroll
         for (int kt = 0; kt < kMassTiles; ++kt) {
-            const int pos = k0 + 16 * kt + c;
-            const int lb = (int)(((uint64_t)(uint32_t)pos * p.bs_magic) >> 40);
-            const int bid = pos < k_hi && lb < p.max_blocks ? table[lb] : -1;
-            ok[kt] = bid >= 0 && (int64_t)bid < p.num_blocks;
-            const int slot = pos - lb * p.block_size;
-            ksc[kt] = p.scale_log2;
-            if (ok[kt]) {
-                load_k<KV, D>(p, (int64_t)bid * p.block_stride + ((int64_t)slot * p.num_kv_heads + kvh) * D, g, k[kt]);
-                if constexpr (SCALED)
-                    ksc[kt] *= (float)__builtin_bit_cast(
-                        _Float16, p.k_scale[(int64_t)bid * p.scale_block_stride + (int64_t)kvh * p.block_size + slot]);
-            } else {
+            const int from = 16 * kt + c;
+            const int64_t row = (int64_t)(uint32_t)__shfl((int)my_row, from) | (int64_t)__shfl((int)(my_row >> 32), from) << 32;
+            if (__shfl((int)have, from)) load_k<KV, D>(p, row, g, k[kt]);
+            else
 #pragma unroll
                 for (int i = 0; i < MD::NS; ++i) k[kt][i] = h8{};
-            }
+        }
+        if (base + STEP < k_hi) bid = block_of(k0 + STEP, slot);
+#pragma unroll
+        for (int kt = 0; kt < kMassTiles; ++kt) {
+            ksc[kt] = p.scale_log2;
+            if constexpr (SCALED) ksc[kt] *= shfl(my_scale, 16 * kt + c);
         }
         const bool masked = k0 + kMassKeys > sq.plain;
         float sum[kMassTiles] = {0.f, 0.f, 0.f, 0.f};
-        for (int r0 = 0; r0 < M; r0 += 16) {
-            h8 q[MD::NS];
-            {
-                const int row = r0 + c, t = row / G;
-                const bool in = row < M;
-                const _Float16* b = reinterpret_cast<const _Float16*>(p.q) +
-                                    ((int64_t)(sq.q0 + (in ? t : 0)) * p.num_heads + kvh * G + (in ? row - t * G : 0)) * D;
-#pragma unroll
-                for (int i = 0; i < MD::NS; ++i)
-                    q[i] = in && (i < MD::NC || g < 2) ? *reinterpret_cast<const h8*>(b + MD::dim(i, g)) : h8{};
+        for (int r0 = 0; r0 < M; r0 += 16 * RBS) {
+            if (several) {
+                __syncthreads();
+                stage(r0);
             }
-            float shift[4];
-            uint64_t win[4];
+            const int rows = min(M - r0, 16 * RBS);
+            if (masked) {
+                for (int i = lane; i < (rows + 15) / 16 * 16; i += kWave) {
+                    const int row = r0 + i, t = row / G;
+                    const uint64_t* mrow = p.mask ? p.mask + (int64_t)(sq.q0 + t) * p.mask_words : nullptr;
+                    win_s[wave][i] = row >= M ? 0
+                                              : (uint64_t)tree_window(p, sq, mrow, t, k0 + 32) << 32 |
+                                                    tree_window(p, sq, mrow, t, k0);
+                }
+                asm volatile("" ::: "memory");  // (one wave's LDS accesses are in order)
+            }
+            for (int rb = 0; rb < (ONE ? 1 : (rows + 15) / 16); ++rb) {
+                h8 q[MD::NS];
+                f4 shift;
+                if constexpr (ONE) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = r0 + 4 * g + r, t = row / G;
-                shift[r] = __builtin_inff();  // (rows past the last, and rows that saw nothing, add exp2(-inf))
-                win[r] = 0;
-                if (row < M) {
-                    const float z = p.lse_in[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)];
-                    if (z != -__builtin_inff()) shift[r] = z * kLog2e;
-                    if (masked) {
-                        const uint64_t* mrow = p.mask ? p.mask + (int64_t)(sq.q0 + t) * p.mask_words : nullptr;
-                        win[r] = (uint64_t)tree_window(p, sq, mrow, t, k0 + 32) << 32 | tree_window(p, sq, mrow, t, k0);
+                    for (int i = 0; i < MD::NS; ++i) q[i] = q1[i];
+                    shift = shift1;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < MD::NS; ++i) q[i] = q_s[rb][i][lane];
+                    shift = *reinterpret_cast<const f4*>(&shift_s[16 * rb + 4 * g]);
+                }
+                f4 x[kMassTiles];
+#pragma unroll
+                for (int kt = 0; kt < kMassTiles; ++kt) {
+                    f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < MD::NS; ++i) acc = mfma32(q[i], k[kt][i], acc);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[kt][r] = fmaf(acc[r], ksc[kt], -shift[r]);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint64_t w = win_s[wave][16 * rb + 4 * g + r] >> c;
+#pragma unroll
+                        for (int kt = 0; kt < kMassTiles; ++kt)
+                            x[kt][r] = (w >> (16 * kt)) & 1 ? x[kt][r] : -__builtin_inff();
                     }
                 }
-            }
 #pragma unroll
-            for (int kt = 0; kt < kMassTiles; ++kt) {
-                f4 acc = {0.f, 0.f, 0.f, 0.f};
+                for (int kt = 0; kt < kMassTiles; ++kt)
 #pragma unroll
-                for (int i = 0; i < MD::NS; ++i) acc = mfma32(q[i], k[kt][i], acc);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float x = fmaf(acc[r], ksc[kt], -shift[r]);
-                    if (masked) x = (win[r] >> (16 * kt + c)) & 1 ? x : -__builtin_inff();
-                    sum[kt] += fast_exp2(x);
-                }
+                    for (int r = 0; r < 4; ++r) sum[kt] += fast_exp2(x[kt][r]);
             }
         }
         // The four lane groups' sums; group g writes tile g.
         float mine = 0.f;
-        bool write = false;
 #pragma unroll
         for (int kt = 0; kt < kMassTiles; ++kt) {
-            float x = sum[kt];
-            x += shfl_xor(x, 32);
-            x += shfl_xor(x, 16);
-            if (g == kt) mine = x, write = ok[kt];
+            float y = sum[kt];
+            y += shfl_xor(y, 32);
+            y += shfl_xor(y, 16);
+            if (g == kt) mine = y;
         }
-        if (write) out[k0 + lane] += mine;
+        if (have) out[k0 + lane] = before + mine;
     }
 }
 
@@ -159,7 +227,10 @@ template <int KV, int D>
 hipError_t launch_mass_dim(const TreeParams& p, hipStream_t stream) {
     const int64_t cells = (int64_t)p.num_seqs * p.parts;
     const int64_t grid = (cells + 7) / 8 * 8 * p.num_kv_heads;
-    mass_kernel<KV, D><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);
+    if (p.max_nodes * p.group <= 16)
+        mass_kernel<KV, D, true><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);
+    else
+        mass_kernel<KV, D, false><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);
     return hipGetLastError();
 }
 
