@@ -22,8 +22,8 @@ namespace {
 // them.  Ranks come from ballots: each wave walks a contiguous run of slots, 64
 // at a time, and only the waves' totals meet in LDS.
 //
-// Keys live in LDS (4 bytes a slot) while they fit; longer rows are read again
-// for every pass.
+// Rows of up to 32768 slots (evict_plan_kernel) keep their keys in LDS; longer
+// ones (evict_plan_long_kernel) read them again for every pass.
 
 constexpr int kPlanLdsKeys = 32768;
 
@@ -37,21 +37,221 @@ struct PlanRow {
         const int32_t x = positions ? positions[slot] : -1;
         return x >= 0 ? (int64_t)x : slot + shift;
     }
-    __device__ __forceinline__ uint32_t key(int slot) const {
-        const int64_t at = position(slot);
-        const float x = scores[slot] + 0.f;  // (-0 ranks with +0)
+    __device__ __forceinline__ uint32_t key_of(float score, int64_t at) const {
+        const float x = score + 0.f;  // (-0 ranks with +0)
         const uint32_t b = __float_as_uint(x);
         if (at < first || at >= last) return 0xFFFFFFFFu;
         return x != x ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
     }
+    __device__ __forceinline__ uint32_t key(int slot) const { return key_of(scores[slot], position(slot)); }
 };
 
-template <int T, bool LDS>
+// The budget-th largest key's digit at bit d, from the histogram of the keys
+// that share the digits above it: one wave, four bins a lane from the top.
+// got: {the digit, keys still to take from its bin, keys in its bin}.
+__device__ __forceinline__ void find_digit(const uint32_t* hist, int left, int lane, uint32_t* got) {
+    int n[4], all = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) all += n[j] = (int)hist[255 - 4 * lane - j];
+    int before = wave_excl_scan(all, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (before < left && before + n[j] >= left) got[0] = 255 - 4 * lane - j, got[1] = left - before, got[2] = n[j];
+        before += n[j];
+    }
+}
+
+__device__ __forceinline__ int mbcnt64(uint64_t m) {  // set bits below this lane
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// At most kPlanLdsKeys slots.  Slots in groups of 64: a group's kept slots are
+// one ballot in LDS, ranks are scans of the groups' counts.  The select ends at
+// the first digit whose whole bin stays (distinct scores: after two of four).
+constexpr int kPlanHoles = 2048;  // holes whose slots are in LDS too
+
+template <int T>
 __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
-    constexpr int W = T / 64;
+    constexpr int W = T / 64, GROUPS = kPlanLdsKeys / 64;
     extern __shared__ uint32_t plan_keys[];
+    __shared__ uint64_t kept_s[GROUPS];
+    __shared__ int hole0[GROUPS], filler0[GROUPS];  // holes and fillers before each group
+    __shared__ int holes_s[kPlanHoles];
+    __shared__ uint32_t hist[4][256];
+    __shared__ uint32_t found[3];
+    __shared__ int total_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int s = blockIdx.x / p.num_kv_heads, h = blockIdx.x - s * p.num_kv_heads;
+    const int len = min(max(p.context_lens[s], 0), p.max_len);
+    const int64_t base = (int64_t)blockIdx.x * p.stride;
+    const int64_t seen = p.seen_lens ? (int64_t)p.seen_lens[s] : (int64_t)len;
+    const PlanRow row{p.scores + base, p.positions ? p.positions + base : nullptr, seen - len, p.keep_first,
+                      seen - p.keep_last};
+    float* so = p.scores_out + base;
+    int32_t* po = p.positions_out ? p.positions_out + base : nullptr;
+    const int budget = p.budget, keep = min(len, budget);
+    if (h == 0 && tid == 0) p.new_lens[s] = keep;
+    const bool cut = len > budget;
+    if (cut)
+        for (int i = tid; i < 4 * 256; i += T) (&hist[0][0])[i] = 0;
+    // The state in front of the budget as it is (holes are overwritten by the
+    // moves), and the keys.  (Eight slots' loads at once: the stores may alias
+    // them, so the compiler would wait for each: 4 x 16384 slots 21 -> PLANL us.)
+    constexpr int AT = 8;
+    for (int i0 = tid; i0 < len; i0 += AT * T) {
+        float x[AT];
+        int32_t at[AT];
+#pragma unroll
+        for (int j = 0; j < AT; ++j) {
+            const int i = min(i0 + j * T, len - 1);
+            x[j] = row.scores[i];
+            at[j] = row.positions ? row.positions[i] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < AT; ++j) {
+            const int i = i0 + j * T;
+            if (i >= len) break;
+            const int pos = at[j] >= 0 ? at[j] : (int)(i + row.shift);
+            if (cut) plan_keys[i] = row.key_of(x[j], pos);
+            if (i < keep) {
+                so[i] = x[j];
+                if (po) po[i] = pos;
+            }
+        }
+    }
+    int count = 0;
+    if (cut) {
+        uint32_t limit = 0, ties = 0;  // keys above `limit` stay, and `ties` of the equal ones, in slot order
+        int left = budget;
+        bool all_equal = false;        // every equal one stays
+        __syncthreads();
+        for (int d = 24, n = 0; d >= 0; d -= 8, ++n) {
+            for (int i = tid; i < len; i += T) {
+                const uint32_t k = plan_keys[i];
+                if (d == 24 || (k ^ limit) >> (d + 8) == 0) atomicAdd(&hist[n][k >> d & 255], 1u);
+            }
+            __syncthreads();
+            if (wave == 0) find_digit(hist[n], left, lane, found);
+            __syncthreads();
+            limit |= found[0] << d;
+            left = (int)found[1];
+            if (found[1] == found[2]) {  // (the last digit: `left` equal keys, all of them kept)
+                all_equal = true;
+                break;
+            }
+        }
+        ties = (uint32_t)left;
+        const int groups = (len + 63) / 64;
+        const auto valid = [&](int g) { return len - 64 * g >= 64 ? ~0ull : (1ull << (len - 64 * g)) - 1; };
+        if (all_equal) {  // key >= limit (digits below the found one are 0)
+            for (int g = wave; g < groups; g += W) {
+                const int i = 64 * g + lane;
+                const uint64_t k = __ballot(i < len && plan_keys[min(i, len - 1)] >= limit);
+                if (lane == 0) kept_s[g] = k;
+            }
+        } else {  // equal keys by their rank: counts of the groups first
+            for (int g = wave; g < groups; g += W) {
+                const int i = 64 * g + lane;
+                const int n = __popcll(__ballot(i < len && plan_keys[min(i, len - 1)] == limit));
+                if (lane == 0) hole0[g] = n;
+            }
+            __syncthreads();
+            if (wave == 0) {
+                int before = 0;
+                for (int g = 0; g < groups; g += 64) {
+                    const int n = g + lane < groups ? hole0[g + lane] : 0, incl = wave_incl_scan(n);
+                    if (g + lane < groups) filler0[g + lane] = before + incl - n;
+                    before += __builtin_amdgcn_readlane(incl, 63);
+                }
+            }
+            __syncthreads();
+            for (int g = wave; g < groups; g += W) {
+                const int i = 64 * g + lane;
+                const uint32_t k = i < len ? plan_keys[i] : 0u;
+                const uint64_t e = __ballot(i < len && k == limit);
+                const bool stays = i < len && (k > limit || (k == limit && filler0[g] + mbcnt64(e) < (int)ties));
+                const uint64_t b = __ballot(stays);
+                if (lane == 0) kept_s[g] = b;
+            }
+        }
+        __syncthreads();
+        const auto in_front = [&](int g) {  // slots of group g below the budget
+            const int n = budget - 64 * g;
+            return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+        };
+        if (wave == 0) {
+            int hb = 0, fb = 0;
+            for (int g = 0; g < groups; g += 64) {
+                const int gl = g + lane;
+                int nh = 0, nf = 0;
+                if (gl < groups) {
+                    const uint64_t k = kept_s[gl], f = in_front(gl);
+                    nh = __popcll(~k & f & valid(gl));
+                    nf = __popcll(k & ~f);
+                }
+                const int ih = wave_incl_scan(nh), jf = wave_incl_scan(nf);
+                if (gl < groups) hole0[gl] = hb + ih - nh, filler0[gl] = fb + jf - nf;
+                hb += __builtin_amdgcn_readlane(ih, 63);
+                fb += __builtin_amdgcn_readlane(jf, 63);
+            }
+            if (lane == 0) total_s = hb;
+        }
+        __syncthreads();
+        count = min(total_s, p.max_moves);
+        int2* moves = p.moves + (int64_t)blockIdx.x * p.max_moves;
+        const bool in_lds = count <= kPlanHoles;
+        for (int g = wave; 64 * g < budget; g += W) {
+            const uint64_t a = ~kept_s[g] & in_front(g) & valid(g);
+            const int r = hole0[g] + mbcnt64(a);
+            if (a >> lane & 1 && r < count) {
+                if (in_lds) holes_s[r] = 64 * g + lane;
+                else moves[r].x = 64 * g + lane;
+            }
+        }
+        __threadfence_block();
+        __syncthreads();
+        constexpr int FG = 4;  // groups at once
+        for (int g0 = budget / 64 + wave; g0 < groups; g0 += FG * W) {
+            float x[FG];
+            int32_t pos[FG];
+            int rank[FG];
+#pragma unroll
+            for (int j = 0; j < FG; ++j) {
+                const int g = g0 + j * W, from = 64 * g + lane;
+                rank[j] = -1;
+                if (g >= groups) continue;
+                const uint64_t b = kept_s[g] & ~in_front(g);
+                const int r = filler0[g] + mbcnt64(b);
+                if (!(b >> lane & 1) || r >= count) continue;
+                rank[j] = r;
+                x[j] = row.scores[from];
+                pos[j] = row.positions ? row.positions[from] : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < FG; ++j) {
+                const int r = rank[j], from = 64 * (g0 + j * W) + lane;
+                if (r < 0) continue;
+                const int to = in_lds ? holes_s[r] : moves[r].x;
+                if (in_lds) moves[r] = make_int2(to, from);
+                else moves[r].y = from;
+                so[to] = x[j];
+                if (po) po[to] = pos[j] >= 0 ? pos[j] : (int)(from + row.shift);
+            }
+        }
+        __syncthreads();  // (scores_out may be scores: sources are read before they are cleared)
+    }
+    if (tid == 0) p.move_counts[blockIdx.x] = count;
+    for (int i = keep + tid; i < p.max_len; i += T) {
+        so[i] = 0.f;
+        if (po) po[i] = -1;
+    }
+}
+
+template <int T>
+__global__ __launch_bounds__(T) void evict_plan_long_kernel(EvictPlanParams p) {
+    constexpr int W = T / 64;
     __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];
+    __shared__ uint32_t found[3];
     __shared__ int tot[3][W];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int s = blockIdx.x / p.num_kv_heads, h = blockIdx.x - s * p.num_kv_heads;
@@ -72,10 +272,7 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
     int ties = 0;        // slots of equal keys that stay, in slot order
     int count = 0;       // moves
     if (len > budget) {
-        if constexpr (LDS) {
-            for (int i = tid; i < len; i += T) plan_keys[i] = row.key(i);
-        }
-        const auto key = [&](int i) { return LDS ? plan_keys[i] : row.key(i); };
+        const auto key = [&](int i) { return row.key(i); };
         int left = budget;
         for (int d = 24; d >= 0; d -= 8) {
             __syncthreads();
@@ -86,18 +283,7 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
                 if (d == 24 || (k ^ limit) >> (d + 8) == 0) atomicAdd(&hist[k >> d & 255], 1u);
             }
             __syncthreads();
-            if (wave == 0) {  // the digit at which the keys from the top reach `left`
-                // lane: digits 255 - 4 lane .. 252 - 4 lane
-                int n[4], all = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) all += n[j] = (int)hist[255 - 4 * lane - j];
-                int before = wave_excl_scan(all, lane);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (before < left && before + n[j] >= left) found[0] = 255 - 4 * lane - j, found[1] = left - before;
-                    before += n[j];
-                }
-            }
+            if (wave == 0) find_digit(hist, left, lane, found);
             __syncthreads();
             limit |= found[0] << d;
             left = (int)found[1];
@@ -115,7 +301,7 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
             const bool in = i + lane < hi;
             const uint32_t k = in ? key(i + lane) : 0u;
             const uint64_t e = __ballot(in && k == limit);
-            const int at = equal + __builtin_amdgcn_mbcnt_hi((uint32_t)(e >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)e, 0));
+            const int at = equal + mbcnt64(e);
             equal += __popcll(e);
             return __ballot(in && (k > limit || (k == limit && at < ties)));
         };
@@ -141,8 +327,8 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
         for (int i = lo; i < hi; i += 64) {
             const uint64_t k = kept(i, equal), f = in_front(i), v = valid(i);
             const uint64_t a = ~k & f & v, b = k & ~f;
-            const int ra = hole + __builtin_amdgcn_mbcnt_hi((uint32_t)(a >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)a, 0));
-            const int rb = filler + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+            const int ra = hole + mbcnt64(a);
+            const int rb = filler + mbcnt64(b);
             if (a >> lane & 1 && ra < p.max_moves) moves[ra].x = i + lane;
             if (b >> lane & 1 && rb < p.max_moves) moves[rb].y = i + lane;
             if (k & f & 1ull << lane) {
@@ -275,15 +461,14 @@ __global__ __launch_bounds__(256) void commit_kernel(RowMoveParams p, int width,
 hipError_t launch_evict_plan(const EvictPlanParams& p, hipStream_t stream) {
     const dim3 grid((uint32_t)(p.num_seqs * p.num_kv_heads));
     if (p.max_len > kPlanLdsKeys) {
-        evict_plan_kernel<1024, false><<<grid, dim3(1024), 0, stream>>>(p);
+        evict_plan_long_kernel<1024><<<grid, dim3(1024), 0, stream>>>(p);
     } else if (p.max_len > 4096) {
-        const int lds = p.max_len * 4;
-        const hipError_t e = hipFuncSetAttribute((const void*)evict_plan_kernel<1024, true>,
+        const hipError_t e = hipFuncSetAttribute((const void*)evict_plan_kernel<1024>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, kPlanLdsKeys * 4);
         if (e != hipSuccess) return e;
-        evict_plan_kernel<1024, true><<<grid, dim3(1024), lds, stream>>>(p);
+        evict_plan_kernel<1024><<<grid, dim3(1024), p.max_len * 4, stream>>>(p);
     } else {
-        evict_plan_kernel<256, true><<<grid, dim3(256), p.max_len * 4, stream>>>(p);
+        evict_plan_kernel<256><<<grid, dim3(256), p.max_len * 4, stream>>>(p);
     }
     return hipGetLastError();
 }
