@@ -90,14 +90,23 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
     // Rows r0 .. r0 + 16 RBS - 1 into LDS.
     auto stage = [&](int r0) {
         const int rows = min(M - r0, 16 * RBS), units = (rows + 15) / 16 * MD::NS * kWave;
-        for (int u = threadIdx.x; u < units; u += 64 * kMassWaves) {
+        constexpr int EACH = (RBS * MD::NS + kMassWaves - 1) / kMassWaves;  // a thread's units, loaded at once
+        h8 v[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const int u = threadIdx.x + 64 * kMassWaves * j;
             const int l = u & 63, i = u / kWave % MD::NS, rb = u / (kWave * MD::NS);
             const int row = r0 + 16 * rb + (l & 15), gg = l >> 4, t = row / G;
-            const bool in = row < M && (i < MD::NC || gg < 2);
-            q_s[rb][i][l] = in ? *reinterpret_cast<const h8*>(
-                                     reinterpret_cast<const _Float16*>(p.q) +
-                                     ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D + MD::dim(i, gg))
-                               : h8{};
+            const bool in = u < units && row < M && (i < MD::NC || gg < 2);
+            v[j] = in ? *reinterpret_cast<const h8*>(
+                            reinterpret_cast<const _Float16*>(p.q) +
+                            ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D + MD::dim(i, gg))
+                      : h8{};
+        }
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const int u = threadIdx.x + 64 * kMassWaves * j;
+            if (u < units) (&q_s[0][0][0])[u] = v[j];
         }
         for (int i = threadIdx.x; i < (rows + 15) / 16 * 16; i += 64 * kMassWaves) {
             const int row = r0 + i, t = row / G;
@@ -121,14 +130,8 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
     const bool several = !ONE && M > 16 * RBS;
     constexpr int STEP = kMassKeys * kMassWaves;
     int slot = 0, bid = block_of(k_lo + kMassKeys * wave, slot);
-    if (!several) stage(0);
     h8 q1[MD::NS];
     f4 shift1 = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (ONE) {
-#pragma unroll
-        for (int i = 0; i < MD::NS; ++i) q1[i] = q_s[0][i][lane];
-        shift1 = *reinterpret_cast<const f4*>(&shift_s[4 * g]);
-    }
     for (int base = k_lo; base < k_hi; base += STEP) {  // (whole workgroup)
         const int k0 = base + kMassKeys * wave;
         const bool have = bid >= 0;
@@ -159,9 +162,14 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
         const bool masked = k0 + kMassKeys > sq.plain;
         float sum[kMassTiles] = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < M; r0 += 16 * RBS) {
-            if (several) {
-                __syncthreads();
+            if (several || base == k_lo) {  // (behind the first K loads)
+                if (r0 > 0 || base > k_lo) __syncthreads();
                 stage(r0);
+                if constexpr (ONE) {
+#pragma unroll
+                    for (int i = 0; i < MD::NS; ++i) q1[i] = q_s[0][i][lane];
+                    shift1 = *reinterpret_cast<const f4*>(&shift_s[4 * g]);
+                }
             }
             const int rows = min(M - r0, 16 * RBS);
             if (masked) {
