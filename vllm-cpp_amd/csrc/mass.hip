@@ -4,13 +4,20 @@
 //
 // With the rows' log-sum-exp given, every position is independent: no running
 // maximum, no merge, and each sum is formed by one wave in a fixed order (no
-// atomics, the same bits every time).  A wave owns KT tiles of 16 positions;
+// atomics, the same bits every time).  A wave owns 64 positions at a time;
 // S[16 rows][16 positions] = Q x K^T comes from 16x16x32 f16 products with the
 // rows along a lane's accumulators, so that a lane sums its position's weights
 // in registers and only the four lane groups meet at the end.  K goes straight
 // from its pages to the product's operands (a lane's 16 bytes are 16 bytes of
-// its position's row): each row of K is read once per kv head.  The rows'
-// operands and log-sum-exps are staged in LDS, 128 rows at a time.
+// its position's row): each row of K is read once per kv head.
+//
+// A decode step (few rows) is bound by the K bytes: their operand stays in
+// registers and the waves of a workgroup take neighbouring heads (64 sequences
+// of 128..4096 fp16 tokens, 64 heads over 8 kv heads of 80: 173 MB cold in 44.5
+// us, 3.9 TB/s with the launch; a head per workgroup 50.2).  Many rows are bound by
+// the products and exponentials: the rows' operands and log-sum-exps are staged
+// in LDS, 128 rows at a time.  K loads a step ahead of the products measured
+// slower in both (59 us and 42 against 50 and 26: the registers cost waves).
 #include "device_common.h"
 #include "tree.h"
 #include "tree_mask.h"
@@ -62,24 +69,29 @@ __device__ __forceinline__ void load_k(const TreeParams& p, int64_t row, int g, 
 // Rows (node, head of the group) held in LDS at a time.
 constexpr int kMassRows = 128;
 
-// ONE: at most 16 rows (a decode step): their operand stays in registers, and
-// the next positions' block ids and scores are loaded beside this one's K.
+// ONE: at most kMassOneRows rows.  The next positions' block ids are loaded
+// beside this step's K.  Four waves a SIMD where the registers allow it without
+// scratch (decode 46.8 -> 44.5 us).
 template <int KV, int D, bool ONE>
-__global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
+__global__ __launch_bounds__(64 * kMassWaves, D == 64 || (ONE && D == 80 && KV == VCPP_KV_F16) ? 4 : 3) void mass_kernel(TreeParams p) {
     using MD = MassDims<KV, D>;
     constexpr bool SCALED = KV == VCPP_KV_I8;
     constexpr int RBS = ONE ? 1 : kMassRows / 16;
-    __shared__ __attribute__((aligned(16))) h8 q_s[RBS][MD::NS][kWave];     // operands as the lanes hold them
+    __shared__ __attribute__((aligned(16))) h8 q_s[ONE ? 1 : RBS][MD::NS][kWave];     // operands as the lanes hold them
     __shared__ __attribute__((aligned(16))) float shift_s[RBS * 16];        // log-sum-exps in log2 units
     __shared__ uint64_t win_s[kMassWaves][RBS * 16];                        // windows of each wave's 64 positions
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     // The kv heads of one (sequence, part) share an XCD (and its L2's lines).
     const int jj = blockIdx.x >> 3;
-    const int cell = (jj / p.num_kv_heads) * 8 + (blockIdx.x & 7);
-    const int kvh = jj % p.num_kv_heads;
-    const int part = cell / p.num_seqs, s = cell - part * p.num_seqs;
-    if (part >= p.parts) return;
+    // ONE: head_waves waves take that many heads next to each other, and the same
+    // positions; else the waves take 64 positions each of one head.
+    const int hw = ONE ? p.head_waves : 1, lanes_of = ONE ? p.num_kv_heads / hw : p.num_kv_heads;
+    const int cell = (jj / lanes_of) * 8 + (blockIdx.x & 7);
+    const int kvh = ONE ? jj % lanes_of * hw + wave % hw : jj % lanes_of;
+    const int at = ONE ? wave / hw : wave;
+    const int s = cell / p.parts, part = cell - s * p.parts;
+    if (s >= p.num_seqs) return;
     const TreeSeq sq(p, s);
     const int G = p.group, M = sq.n * G;
     const int k_lo = part * p.part_len, k_hi = min(k_lo + p.part_len, sq.end);
@@ -87,36 +99,39 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
     const int32_t* table = p.block_tables + (int64_t)s * p.max_blocks;
     float* out = p.scores + ((int64_t)s * p.num_kv_heads + kvh) * p.score_stride;
 
+    // Slice i of lane group gg of a row's operand, and the row's log-sum-exp in
+    // log2 units (rows past the last, and rows that saw nothing, add exp2(-inf)).
+    auto q_of = [&](int row, int i, int gg) {
+        const int t = row / G;
+        return row < M && (i < MD::NC || gg < 2)
+                   ? *reinterpret_cast<const h8*>(
+                         reinterpret_cast<const _Float16*>(p.q) +
+                         ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D + MD::dim(i, gg))
+                   : h8{};
+    };
+    auto shift_of = [&](int row) {
+        const int t = row / G;
+        const float x = row < M ? p.lse_in[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)]
+                                : -__builtin_inff();
+        return x != -__builtin_inff() ? x * kLog2e : __builtin_inff();
+    };
     // Rows r0 .. r0 + 16 RBS - 1 into LDS.
     auto stage = [&](int r0) {
-        const int rows = min(M - r0, 16 * RBS), units = (rows + 15) / 16 * MD::NS * kWave;
+        const int units = (min(M - r0, 16 * RBS) + 15) / 16 * MD::NS * kWave;
         constexpr int EACH = (RBS * MD::NS + kMassWaves - 1) / kMassWaves;  // a thread's units, loaded at once
         h8 v[EACH];
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             const int u = threadIdx.x + 64 * kMassWaves * j;
             const int l = u & 63, i = u / kWave % MD::NS, rb = u / (kWave * MD::NS);
-            const int row = r0 + 16 * rb + (l & 15), gg = l >> 4, t = row / G;
-            const bool in = u < units && row < M && (i < MD::NC || gg < 2);
-            v[j] = in ? *reinterpret_cast<const h8*>(
-                            reinterpret_cast<const _Float16*>(p.q) +
-                            ((int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)) * D + MD::dim(i, gg))
-                      : h8{};
+            v[j] = u < units ? q_of(r0 + 16 * rb + (l & 15), i, l >> 4) : h8{};
         }
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             const int u = threadIdx.x + 64 * kMassWaves * j;
             if (u < units) (&q_s[0][0][0])[u] = v[j];
         }
-        for (int i = threadIdx.x; i < (rows + 15) / 16 * 16; i += 64 * kMassWaves) {
-            const int row = r0 + i, t = row / G;
-            float z = __builtin_inff();  // (rows past the last, and rows that saw nothing, add exp2(-inf))
-            if (row < M) {
-                const float x = p.lse_in[(int64_t)(sq.q0 + t) * p.num_heads + kvh * G + (row - t * G)];
-                if (x != -__builtin_inff()) z = x * kLog2e;
-            }
-            shift_s[i] = z;
-        }
+        for (int i = threadIdx.x; i < RBS * 16; i += 64 * kMassWaves) shift_s[i] = shift_of(r0 + i);
         __syncthreads();
     };
     // This lane's position of the wave's 64 at k0: its block id (-1: none).
@@ -128,12 +143,12 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
         return bid >= 0 && (int64_t)bid < p.num_blocks ? bid : -1;
     };
     const bool several = !ONE && M > 16 * RBS;
-    constexpr int STEP = kMassKeys * kMassWaves;
-    int slot = 0, bid = block_of(k_lo + kMassKeys * wave, slot);
+    const int step = kMassKeys * kMassWaves / hw;
+    int slot = 0, bid = block_of(k_lo + kMassKeys * at, slot);
     h8 q1[MD::NS];
     f4 shift1 = {0.f, 0.f, 0.f, 0.f};
-    for (int base = k_lo; base < k_hi; base += STEP) {  // (whole workgroup)
-        const int k0 = base + kMassKeys * wave;
+    for (int base = k_lo; base < k_hi; base += step) {  // (whole workgroup)
+        const int k0 = base + kMassKeys * at;
         const bool have = bid >= 0;
         h8 k[kMassTiles][MD::NS];
         float ksc[kMassTiles];
@@ -153,7 +168,7 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
 #pragma unroll
                 for (int i = 0; i < MD::NS; ++i) k[kt][i] = h8{};
         }
-        if (base + STEP < k_hi) bid = block_of(k0 + STEP, slot);
+        if (base + step < k_hi) bid = block_of(k0 + step, slot);
 #pragma unroll
         for (int kt = 0; kt < kMassTiles; ++kt) {
             ksc[kt] = p.scale_log2;
@@ -162,14 +177,16 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
         const bool masked = k0 + kMassKeys > sq.plain;
         float sum[kMassTiles] = {0.f, 0.f, 0.f, 0.f};
         for (int r0 = 0; r0 < M; r0 += 16 * RBS) {
-            if (several || base == k_lo) {  // (behind the first K loads)
+            if constexpr (ONE) {
+                if (base == k_lo) {  // (behind the first K loads)
+#pragma unroll
+                    for (int i = 0; i < MD::NS; ++i) q1[i] = q_of(c, i, g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) shift1[r] = shift_of(4 * g + r);
+                }
+            } else if (several || base == k_lo) {
                 if (r0 > 0 || base > k_lo) __syncthreads();
                 stage(r0);
-                if constexpr (ONE) {
-#pragma unroll
-                    for (int i = 0; i < MD::NS; ++i) q1[i] = q_s[0][i][lane];
-                    shift1 = *reinterpret_cast<const f4*>(&shift_s[4 * g]);
-                }
             }
             const int rows = min(M - r0, 16 * RBS);
             if (masked) {
@@ -234,8 +251,9 @@ __global__ __launch_bounds__(64 * kMassWaves) void mass_kernel(TreeParams p) {
 template <int KV, int D>
 hipError_t launch_mass_dim(const TreeParams& p, hipStream_t stream) {
     const int64_t cells = (int64_t)p.num_seqs * p.parts;
-    const int64_t grid = (cells + 7) / 8 * 8 * p.num_kv_heads;
-    if (p.max_nodes * p.group <= 16)
+    const bool one = p.max_nodes * p.group <= kMassOneRows;
+    const int64_t grid = (cells + 7) / 8 * 8 * (one ? p.num_kv_heads / p.head_waves : p.num_kv_heads);
+    if (one)
         mass_kernel<KV, D, true><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);
     else
         mass_kernel<KV, D, false><<<dim3((uint32_t)grid), dim3(64 * kMassWaves), 0, stream>>>(p);

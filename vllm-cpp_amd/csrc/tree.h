@@ -54,6 +54,7 @@ struct TreeParams {
     // Position split (weights): parts of part_len positions.
     int32_t part_len;
     int32_t parts;
+    int32_t head_waves;  // kv heads of a workgroup where a head has at most kMassOneRows rows (divides num_kv_heads)
     // weights: each row's log-sum-exp and the sums [num_seqs][num_kv_heads][score_stride]
     const float* lse_in;
     float* scores;
@@ -63,6 +64,8 @@ struct TreeParams {
 // Key blocks (32 positions) of a range, at least: a call that has fewer is cut
 // into fewer ranges.
 constexpr int kTreeMinBlocks = 4;
+// Rows of a kv head up to which a wave of the weights' kernel keeps them in registers.
+constexpr int kMassOneRows = 16;
 // Rows (node, head of the group) of one workgroup for trees of `rows` rows.
 int tree_tile_rows(int kv_dtype, int head_dim, int rows);
 // Workgroups of that tile a CU holds at once.
