@@ -381,6 +381,7 @@ int vcpp_kv_evict_plan(const float* scores, const int32_t* positions, int64_t st
  * (a plan's never are); moves from or to a missing block are skipped.  The
  * sequences must not share the blocks in question (copy shared prefixes
  * first).  Blocks past new_lens are then free to be returned.  Any page dtype.
+ * max_moves <= 2^24.
  */
 int vcpp_kv_evict_apply(const vcpp_kv_pages* kv, const int32_t* block_tables, int32_t max_blocks_per_seq,
                         const int32_t* moves, int32_t max_moves, const int32_t* move_counts, int32_t num_seqs,

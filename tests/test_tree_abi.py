@@ -148,6 +148,7 @@ def test_plan_refusals(kw, code, frag):
     (dict(moves=None), INV, "NULL"),
     (dict(counts=None), INV, "NULL"),
     (dict(n=-1), INV, "max_moves"),
+    (dict(n=2**24 + 1), UNS, "max_moves"),
     (dict(moves=P + 4), INV, "aligned"),
     (dict(seqs=9000), UNS, "too many"),
 ])

@@ -342,6 +342,7 @@ int vcpp_kv_evict_apply(const vcpp_kv_pages* kv, const int32_t* block_tables, in
     const int rc = move_params(kv, block_tables, max_blocks_per_seq, num_seqs, p);
     if (rc != VCPP_OK) return rc;
     if (max_moves < 0) return fail(VCPP_E_INVALID, "max_moves must be >= 0");
+    if (max_moves > kMaxLen) return fail(VCPP_E_UNSUPPORTED, "max_moves %d too many", max_moves);
     if ((int64_t)num_seqs * kv->num_kv_heads > 65535) return fail(VCPP_E_UNSUPPORTED, "too many sequences x kv heads");
     if (num_seqs == 0 || max_moves == 0) return VCPP_OK;
     if (!moves || !move_counts) return fail(VCPP_E_INVALID, "moves/move_counts is NULL");

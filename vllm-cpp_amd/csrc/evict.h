@@ -45,7 +45,6 @@ struct RowMoveParams {
     int32_t row_bytes;          // of one head's row
     int32_t scaled;             // int8 pages
     int32_t num_layers;
-    uint64_t bs_magic;          // pos / block_size = (pos * bs_magic) >> 40
     const int32_t* block_tables;
     int32_t max_blocks;
     int32_t num_seqs;

@@ -68,7 +68,13 @@ __device__ __forceinline__ int mbcnt64(uint64_t m) {  // set bits below this lan
 // At most kPlanLdsKeys slots.  Slots in groups of 64: a group's kept slots are
 // one ballot in LDS, ranks are scans of the groups' counts.  The select ends at
 // the first digit whose whole bin stays (distinct scores: after two of four).
-constexpr int kPlanHoles = 2048;  // holes whose slots are in LDS too
+//
+// The first digit is a score's sign and seven bits of its exponent: most scores
+// share a few bins, and LDS atomics on one word queue up.  Its histogram is
+// counted while the keys are made, in kPlanCopies copies on different banks.
+constexpr int kPlanCopies = 8;
+constexpr int kPlanCopy = 257;                        // words of a copy
+constexpr int kPlanHoles = kPlanCopies * kPlanCopy;   // holes whose slots are in LDS too (behind the select)
 
 template <int T>
 __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
@@ -76,8 +82,9 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
     extern __shared__ uint32_t plan_keys[];
     __shared__ uint64_t kept_s[GROUPS];
     __shared__ int hole0[GROUPS], filler0[GROUPS];  // holes and fillers before each group
-    __shared__ int holes_s[kPlanHoles];
+    __shared__ int holes_s[kPlanHoles];  // (first the first digit's histograms)
     __shared__ uint32_t hist[4][256];
+    uint32_t* const copies = reinterpret_cast<uint32_t*>(holes_s);
     __shared__ uint32_t found[3];
     __shared__ int total_s;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -92,11 +99,14 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
     const int budget = p.budget, keep = min(len, budget);
     if (h == 0 && tid == 0) p.new_lens[s] = keep;
     const bool cut = len > budget;
-    if (cut)
+    if (cut) {
         for (int i = tid; i < 4 * 256; i += T) (&hist[0][0])[i] = 0;
+        for (int i = tid; i < kPlanHoles; i += T) copies[i] = 0;
+        __syncthreads();
+    }
     // The state in front of the budget as it is (holes are overwritten by the
-    // moves), and the keys.  (Eight slots' loads at once: the stores may alias
-    // them, so the compiler would wait for each: 4 x 16384 slots 21 -> PLANL us.)
+    // moves), and the keys.  (Eight slots are loaded before any is stored: the
+    // stores may alias the loads, so that the compiler keeps their order.)
     constexpr int AT = 8;
     for (int i0 = tid; i0 < len; i0 += AT * T) {
         float x[AT];
@@ -112,7 +122,11 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
             const int i = i0 + j * T;
             if (i >= len) break;
             const int pos = at[j] >= 0 ? at[j] : (int)(i + row.shift);
-            if (cut) plan_keys[i] = row.key_of(x[j], pos);
+            if (cut) {
+                const uint32_t k = row.key_of(x[j], pos);
+                plan_keys[i] = k;
+                atomicAdd(&copies[tid % kPlanCopies * kPlanCopy + (k >> 24)], 1u);
+            }
             if (i < keep) {
                 so[i] = x[j];
                 if (po) po[i] = pos;
@@ -126,9 +140,18 @@ __global__ __launch_bounds__(T) void evict_plan_kernel(EvictPlanParams p) {
         bool all_equal = false;        // every equal one stays
         __syncthreads();
         for (int d = 24, n = 0; d >= 0; d -= 8, ++n) {
-            for (int i = tid; i < len; i += T) {
-                const uint32_t k = plan_keys[i];
-                if (d == 24 || (k ^ limit) >> (d + 8) == 0) atomicAdd(&hist[n][k >> d & 255], 1u);
+            if (d == 24) {
+                if (tid < 256) {
+                    uint32_t sum = 0;
+#pragma unroll
+                    for (int c = 0; c < kPlanCopies; ++c) sum += copies[c * kPlanCopy + tid];
+                    hist[0][tid] = sum;
+                }
+            } else {
+                for (int i = tid; i < len; i += T) {
+                    const uint32_t k = plan_keys[i];
+                    if ((k ^ limit) >> (d + 8) == 0) atomicAdd(&hist[n][k >> d & 255], 1u);
+                }
             }
             __syncthreads();
             if (wave == 0) find_digit(hist[n], left, lane, found);
@@ -374,9 +397,9 @@ __global__ __launch_bounds__(T) void evict_plan_long_kernel(EvictPlanParams p) {
 // false where the table or the pool has none.
 __device__ __forceinline__ bool place(const RowMoveParams& p, const int32_t* table, int64_t pos, int& bid, int& at) {
     if (pos < 0 || pos >= (int64_t)p.max_blocks * p.block_size) return false;
-    const int lb = (int)(pos / p.block_size);
+    const uint32_t x = (uint32_t)pos, lb = x / (uint32_t)p.block_size;  // (positions are below 2^31 + 256)
     bid = table[lb];
-    at = (int)(pos - (int64_t)lb * p.block_size);
+    at = (int)(x - lb * (uint32_t)p.block_size);
     return bid >= 0 && (int64_t)bid < p.num_blocks;
 }
 
@@ -385,11 +408,13 @@ __device__ __forceinline__ bool place(const RowMoveParams& p, const int32_t* tab
 __global__ __launch_bounds__(256) void evict_apply_kernel(RowMoveParams p) {
     const int s = blockIdx.y / p.num_kv_heads, h = blockIdx.y - s * p.num_kv_heads;
     const int pieces = p.row_bytes / 16, per = 2 * pieces;  // K's, then V's
-    const int count = min(p.move_counts[blockIdx.y], p.max_moves);
+    const int count = min(max(p.move_counts[blockIdx.y], 0), p.max_moves);
     const int32_t* table = p.block_tables + (int64_t)s * p.max_blocks;
     const int2* moves = p.moves + (int64_t)blockIdx.y * p.max_moves;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)count * per; i += (int64_t)gridDim.x * 256) {
-        const int j = (int)(i / per), piece = (int)(i - (int64_t)j * per);
+    // (32-bit indexes and divisions: 0 .. 2^24 moves of at most 64 pieces.)
+    const uint32_t items = (uint32_t)count * (uint32_t)per;
+    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < items; i += gridDim.x * 256u) {
+        const int j = (int)(i / (uint32_t)per), piece = (int)(i - (uint32_t)(j * per));
         const int2 m = moves[j];
         int tb, ta, fb, fa;
         if (!place(p, table, m.x, tb, ta) || !place(p, table, m.y, fb, fa)) continue;
