@@ -84,6 +84,35 @@ def test_mass_any_mask_and_rows_that_see_nothing(p):
     check_mass("f16", 8, 2, 80, 16, [p, 10], [40, 3], kind="any", seed=5)
 
 
+@pytest.mark.parametrize("kv", ["f16", "i8", "fp8"])
+@pytest.mark.parametrize("hkv", [1, 2, 3, 4, 6, 12])
+def test_mass_of_a_decode_step(kv, hkv):
+    """One query a sequence, head counts that fill a workgroup's waves and do not."""
+    check_mass(kv, 2 * hkv, hkv, 80, 16, [300, 0, 64, 1025, 17], [1, 1, 1, 1, 0], seed=hkv)
+
+
+@pytest.mark.parametrize("kv", ["f16", "i8"])
+def test_mass_moves_and_commit_past_32_bits(kv):
+    """Blocks 2^30 elements apart: byte offsets past 2^32, the dense pool's bits."""
+    pool = U.Pool(kv, [70], 2, 80, 16, seed=2, extra=0)
+    q, lse = torch.randn(10, 8, 80).half(), torch.full((10, 8), 5.0)
+    base = torch.rand(1, 2, 70)
+    want = mass(pool, q, lse, base, [60], [10], None, 8)
+    got, tables = base.to(DEV), pool.tables.to(DEV)
+    far, room = U.far(pool, DEV)
+    pyvcpp.attention_mass(far, q.to(DEV), lse.to(DEV), got, tables, dev([0, 10]), dev([60]), 10, 60, 8)
+    assert torch.equal(got.cpu(), want)
+    pages, b = pool.to(DEV)
+    moves, counts = dev([[[[1, 69], [17, 40]], [[0, 33], [2, 65]]]]), dev([[2, 2]])
+    for x in (pages, far):
+        pyvcpp.kv_evict_apply(x, tables, moves, counts)
+        pyvcpp.kv_commit(x, tables, dev([40]), dev([[3, 29, 20]]), dev([3]), 30)
+    torch.cuda.synchronize()
+    for n in b:
+        assert not torch.equal(b[n].cpu(), getattr(pool, n))
+        assert torch.equal(torch.stack([r.view(b[n].dtype) for r in U.near(room, n, pool)]).reshape(b[n].shape), b[n])
+
+
 def test_mass_missing_blocks_and_masked_rows():
     """Positions of missing blocks keep their scores; a drafted K row of NaN
     counts only where it is seen."""

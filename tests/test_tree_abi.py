@@ -84,6 +84,9 @@ def test_tree_and_mass_refusals(fn, kw, code, frag):
     (dict(prefix=100000, ws=P, nws=16), WS, "workspace"),
     (dict(prefix=100000, ws=P + 4, nws=2**40), INV, "workspace"),
     (dict(seqs=2**24, nodes=200, words=4), UNS, "too many"),
+    (dict(pg=pages(hkv=40000, d=128), heads=40000), UNS, "kv heads"),
+    (dict(pg=pages(hkv=1), heads=65535, nodes=256, words=4, prefix=2**24 - 256, seqs=1), UNS, "positions"),
+    (dict(pg=pages(hkv=1), heads=4096, nodes=256, words=4, prefix=2**20, seqs=64), UNS, "positions"),
 ])
 def test_tree_refusals(kw, code, frag):
     assert tree(**kw) == code

@@ -106,6 +106,15 @@ def test_ragged_batch_with_empty_sequences(kv):
 
 
 @pytest.mark.parametrize("kv", ["f16", "i8", "fp8"])
+@pytest.mark.parametrize("seqs", [64, 65, 150])
+def test_many_sequences(kv, seqs):
+    """More sequences than lanes, most of them short, some empty, one long."""
+    prefix = [(37 * s) % 90 for s in range(seqs)]
+    prefix[seqs - 2] = 1500
+    check(kv, 4, 2, 80, 16, prefix, [(5 * s) % 7 for s in range(seqs)], seed=4)
+
+
+@pytest.mark.parametrize("kv", ["f16", "i8", "fp8"])
 @pytest.mark.parametrize("p", [0, 20, 64])
 def test_any_mask_and_empty_rows(kv, p):
     """Masks that are no trees, rows that see no node; at prefix 0 those are zeros with lse -inf."""
@@ -284,6 +293,61 @@ def test_layer_slab_of_a_pool_of_layers():
     want, zw, _ = U.reference(pool, q, [114], [6], U.tree_bits(6, 0, "chain"))
     close(out.cpu(), want)
     close(lse.cpu(), zw)
+
+
+@pytest.mark.parametrize("kv", ["f16", "i8", "fp8"])
+def test_pages_past_32_bits(kv):
+    """Blocks 2^30 elements apart: byte offsets past 2^32, the dense pool's bits."""
+    prefix, nodes = [60, 9], [10, 4]
+    pool = U.Pool(kv, [70, 13], 2, 80, 16, seed=2, extra=0)
+    q = torch.randn(14, 8, 80).half()
+    want = call(pool, q, prefix, nodes, None, 8)
+    pages, keep = U.far(pool, DEV)
+    out, lse = torch.zeros(14, 8, 80, device=DEV), torch.zeros(14, 8, device=DEV)
+    pyvcpp.paged_tree_attention(pages, q.to(DEV), out, pool.tables.to(DEV),
+                                torch.tensor([0, 10, 14], dtype=torch.int32, device=DEV),
+                                torch.tensor(prefix, dtype=torch.int32, device=DEV), 10, 60, 8, lse=lse)
+    torch.cuda.synchronize()
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(lse.cpu(), want[1])
+
+
+def test_byte_pages_on_8_byte_bases():
+    """FP8 pages need 8-byte bases only: the aligned pool's bits."""
+    pool = U.Pool("fp8", [300], 2, 80, 16, seed=2)
+    q = torch.randn(10, 8, 80).half()
+    want = call(pool, q, [290], [10], None, 8)
+    pages, b = pool.to(DEV)
+    room = {n: torch.zeros(b[n].numel() + 16, dtype=torch.uint8, device=DEV) for n in ("k", "v")}
+    for n in room:
+        room[n][8:8 + b[n].numel()] = b[n].flatten()
+    view = pyvcpp.KVPages(pages.dtype, 16, 2, 80, pool.nb, 16 * 2 * 80, 0, room["k"].data_ptr() + 8, room["v"].data_ptr() + 8,
+                          None, None)
+    out, lse = torch.zeros(10, 8, 80, device=DEV), torch.zeros(10, 8, device=DEV)
+    pyvcpp.paged_tree_attention(view, q.to(DEV), out, pool.tables.to(DEV), torch.tensor([0, 10], dtype=torch.int32, device=DEV),
+                                torch.tensor([290], dtype=torch.int32, device=DEV), 10, 290, 8, lse=lse)
+    torch.cuda.synchronize()
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(lse.cpu(), want[1])
+
+
+def test_given_stream_without_a_workspace():
+    """`stream` other than the current one: the scratch that the call allocates
+    stays its own while tensors come and go on the current stream."""
+    pool = U.Pool("f16", [5000], 2, 80, 16, seed=2)
+    q = torch.randn(9, 8, 80).half()
+    want = call(pool, q, [4991], [9], None, 8)
+    pages, keep = pool.to(DEV)
+    args = (q.to(DEV), pool.tables.to(DEV), torch.tensor([0, 9], dtype=torch.int32, device=DEV),
+            torch.tensor([4991], dtype=torch.int32, device=DEV))
+    need = pyvcpp.tree_workspace_size(pages, 1, 9, 4991, 8)
+    outs = [torch.zeros(9, 8, 80, device=DEV) for _ in range(8)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for o in outs:
+        pyvcpp.paged_tree_attention(pages, args[0], o, args[1], args[2], args[3], 9, 4991, 8, stream=side)
+        torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o.cpu(), want[0])
 
 
 def test_workspace_exact_and_garbage():

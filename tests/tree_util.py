@@ -68,6 +68,30 @@ class Pool:
         return out, ok
 
 
+FAR = 1 << 30  # elements between the blocks of `far`
+
+
+def far(pool, device):
+    """(descriptor, buffers) of one layer's pool with its blocks FAR elements apart."""
+    b = {}
+    for n in ("k", "v", "ks", "vs"):
+        t = getattr(pool, n)
+        if t is None:
+            continue
+        t = t.to(device).reshape(pool.nb, -1)
+        b[n] = torch.empty((pool.nb - 1) * FAR + t.shape[1], dtype=t.dtype, device=device)
+        for i in range(pool.nb):
+            b[n][i * FAR:i * FAR + t.shape[1]] = t[i]
+    return pyvcpp.kv_pages(KV[pool.kv], b["k"], b["v"], pool.bs, pool.hkv, pool.D, pool.nb, FAR, b.get("ks"), b.get("vs"),
+                           FAR if pool.kv == "i8" else 0), b
+
+
+def near(buffers, n, pool):
+    """The blocks of a buffer of `far`."""
+    size = getattr(pool, n).reshape(pool.nb, -1).shape[1]
+    return [buffers[n][i * FAR:i * FAR + size] for i in range(pool.nb)]
+
+
 def tree_bits(n, seed, kind="tree"):
     """Ancestor sets as integers: a random tree, a chain, or arbitrary rows
     (some empty)."""

@@ -25,7 +25,7 @@ namespace {
 static_assert(vcpp::kMaxTreeNodes == VCPP_MAX_TREE_NODES, "tree size");
 
 // Longest context of these calls: pos / block_size as a product (tree.h) stays
-// below 2^63, and 64 sequences' key blocks below 2^31.
+// below 2^63.
 constexpr int64_t kMaxLen = 1 << 24;
 
 int fail(int code, const char* fmt, ...) {
@@ -43,6 +43,7 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Cut of a tree call (TreeRanges) and the partials' place in the workspace.
 struct TreeSplit {
+    int64_t blocks;  // of one sequence's row tiles
     int32_t ranges, table_cap;
     size_t off_ml, bytes;
 };
@@ -58,7 +59,8 @@ TreeSplit tree_split(const vcpp_kv_pages* kv, int32_t num_seqs, int32_t max_node
     const int rows = max_nodes * (num_heads / kv->num_kv_heads);
     const int tile = vcpp::tree_tile_rows(kv->dtype, kv->head_dim, rows);
     const int64_t blocks = ((int64_t)max_prefix_len + max_nodes + 31) / 32;
-    const int64_t most = (int64_t)num_seqs * ((rows + tile - 1) / tile) * blocks;  // upper bound of the axis
+    t.blocks = (rows + tile - 1) / tile * blocks;
+    const int64_t most = num_seqs * t.blocks;  // upper bound of the axis
     const int64_t slots = (int64_t)vcpp::compute_units() * vcpp::tree_wgs_per_cu(kv->dtype, kv->head_dim, rows);
     int64_t R = std::min(std::max<int64_t>(1, slots / kv->num_kv_heads), std::max<int64_t>(1, most / vcpp::kTreeMinBlocks));
     // (a piece is no longer than its sequence, nor than its range)
@@ -191,7 +193,13 @@ int vcpp_paged_tree_attention(const vcpp_kv_pages* kv, const uint16_t* q, float*
     if (rc != VCPP_OK || num_seqs == 0 || max_nodes == 0) return rc;
     if (!out) return fail(VCPP_E_INVALID, "out is NULL");
     if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return fail(VCPP_E_INVALID, "out must be 16-byte aligned");
+    // (32-bit places: a row's byte offset in its 16-position tile, 27 bits, and
+    // the key blocks of 64 sequences' row tiles)
+    if ((int64_t)kv->num_kv_heads * kv->head_dim * (kv->dtype == VCPP_KV_F16 ? 2 : 1) > 1 << 23)
+        return fail(VCPP_E_UNSUPPORTED, "too many kv heads (%d of %d dims)", kv->num_kv_heads, kv->head_dim);
     const TreeSplit t = tree_split(kv, num_seqs, max_nodes, max_prefix_len, num_heads);
+    if (t.blocks * std::min(num_seqs, 64) > INT32_MAX)
+        return fail(VCPP_E_UNSUPPORTED, "too many heads or positions for one launch");
     if (!grid_fits(t.ranges, kv->num_kv_heads, 256) || !grid_fits((int64_t)num_seqs * max_nodes, 1, 256))
         return fail(VCPP_E_UNSUPPORTED, "too many sequences, heads or positions for one launch");
     if (t.bytes > 0 && (!workspace || workspace_bytes < t.bytes))

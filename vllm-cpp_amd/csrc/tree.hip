@@ -8,10 +8,13 @@
 // blocks) and zeros (lse -inf) for a row that sees nothing.
 //
 // Work decomposition: the rows of one kv head (node-major, its group's heads
-// next to each other) are cut into tiles of WR waves x RB blocks of 16 rows,
-// the positions into parts of part_len; a workgroup owns (sequence, part, kv
-// head, row tile).  Keys stream in blocks of 32 through a ring of LDS stages
-// filled by direct-to-LDS DMA.  Per key block and 16 rows:
+// next to each other) are cut into tiles of WR waves x RB blocks of 16 rows.
+// All units (sequence, row tile), each as long as its 32-key blocks, lie on one
+// axis that is cut into equal ranges, one per workgroup the GPU holds and kv
+// head (tree_mask.h): uneven sequences cost no one a tail.  A unit that range
+// ends cut leaves partial results (exponent, sum, outputs) in the workspace,
+// which a second kernel merges.  Keys stream through a ring of LDS stages filled
+// by direct-to-LDS DMA.  Per key block and 16 rows:
 //   S^T[32 keys][16 rows] = K x Q^T   (16x16x32 f16)
 //   P = exp2(S scale - m)             (fp32)
 //   O[16 rows][D] += P x V            (16x16x32 f16, twice)
@@ -21,6 +24,12 @@
 // The running exponent leaves 11 bits of headroom below fp16's largest power
 // (P <= 2^15), so that the low part of a P of 2^-16 of the row's largest still
 // has 19 bits; it moves when a row's largest score grows by more than 2^4.
+// What bounds it, 64 heads over 8 kv heads of 80: 16 nodes on 32 fp16 sequences
+// of 128..4096 take 84 us, of which the bytes alone are 49 (173 MB by the ring
+// without products) and the merge 12; 64 nodes on 8 FP8 sequences of 8000..16384
+// take 250 us, of which the products (three per key and row: S, P's high and low
+// part) are 108 at a large matrix product's rate, and the rest the softmax and
+// the widening on the vector units beside them.
 // int8 pages: K and V are exact fp16 integers; the key's K scale multiplies
 // the score, its V scale P (whose exponent is lowered by a running power of two
 // at or above the scales, so that any scale keeps the product in range).
@@ -268,10 +277,10 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
     // DMA: instruction j = wave + WR i fills slots 64 j + lane of a stage, K's
     // rows and then V's, NCHB 16-byte chunks each: neighbouring lanes read
     // neighbouring bytes.  (Chunks key by key, as prefill_tile lays them out,
-    // make every lane of an instruction a request of its own: 64 nodes on
-    // 8000..16384 FP8 tokens 290 -> NEWL us.)  lo: the lane's byte offset in its
-    // tile, its row in the top 5 bits.  Positions past the piece and missing
-    // tiles read zeros.
+    // make every lane of an instruction a request of its own: one node on
+    // 64 fp16 sequences of 128..4096 tokens 101 -> 87 us.)  lo: the lane's byte
+    // offset in its tile, its row in the top 5 bits.  Positions past the piece
+    // and missing tiles read zeros.
     const int my_inst = T::NINST % WR == 0 || wave < T::NINST % WR ? T::PERW : T::PERW - 1;
     const uint32_t row_bytes = (uint32_t)p.num_kv_heads * D * (BYTES ? 1 : 2);
     constexpr int NCHB = BYTES ? ID::NCH : DD::NCH, REGB = kKBlk * NCHB;
@@ -802,7 +811,7 @@ hipError_t launch_tile(const TreeParams& p, hipStream_t stream) {
     if (e != hipSuccess || p.ranges == 1) return e;
     // Ranges per unit, where the sequences are as long as their bound: above 6
     // a wave per row (of about 8192), else a thread per 4 dims (3 pieces, 512
-    // rows of 64 heads: FEWL us against 21).
+    // rows of 64 heads: 12.5 us against 21).
     const int64_t rows = (int64_t)p.num_seqs * p.max_nodes;
     const int64_t units = (int64_t)p.num_seqs * ((p.max_nodes * p.group + ROWS - 1) / ROWS);
     if (p.ranges <= 6 * units) {

@@ -347,6 +347,8 @@ def paged_tree_attention(pages, q, out, block_tables, q_start, prefix_lens, max_
         import torch
         need = tree_workspace_size(pages, S, max_nodes, max_prefix_len, num_heads)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        if stream is not None and workspace is not None:
+            workspace.record_stream(stream)  # (allocated for the current stream)
     _check(lib().vcpp_paged_tree_attention(
         ctypes.byref(pages), op("q", q, op.f16, (rows, num_heads, pages.head_dim)), op("out", out, op.f32, shape),
         op("lse", lse, op.f32, (rows, num_heads)), op("block_tables", block_tables, op.i32, (S, blocks)), blocks,
