@@ -438,31 +438,15 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
             return *reinterpret_cast<__attribute__((address_space(3))) const f4*>(lds + rd_at + ID::SCALES +
                                                                                   ((v ? 32 : 0) + 16 * kt + 4 * g) * 4);
         };
+        f4 ks[2];
+        float top = 0.f;
         if constexpr (SCALED) {
-            float top = 0.f;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
+                ks[kt] = scale4(kt, false);
                 const f4 b = scale4(kt, true);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(b[r]) < 65536.f ? fabsf(b[r]) : 0.f);  // (finite ones)
-            }
-            if (__builtin_expect(__any(top > vcap), 0)) {
-                asm volatile("" : "+v"(top));  // (a branch: as selects its products run for every block)
-                top = fmaxf(top, shfl_xor(top, 16));
-                top = fmaxf(top, shfl_xor(top, 32));
-                const uint32_t up = (__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u;  // (fp16 scales are normal in fp32)
-                const float cap = fmaxf(__uint_as_float(up), vcap);
-                const float down = vcap / cap, by = (float)((int)(__float_as_uint(cap) >> 23) - 127) - vexp;
-                vcap = cap;
-                vexp += by;
-                p_top = kTopP / cap;
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    m_run[rb] += by;
-                    lsum[rb] *= down;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) o[rb][t] *= down;
-                }
             }
         }
         // Bits 16 kt + r: key 16 kt + 4 g + r is seen by row c of row block rb.
@@ -502,14 +486,32 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
                     vb[t] = h8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 }
             }
+            // (behind the first products: the scales' way out of LDS is covered)
+            if (SCALED && r0 == 0 && __builtin_expect(__any(top > vcap), 0)) {
+                asm volatile("" : "+v"(top));  // (a branch: as selects its products run for every block)
+                top = fmaxf(top, shfl_xor(top, 16));
+                top = fmaxf(top, shfl_xor(top, 32));
+                const uint32_t up = (__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u;  // (fp16 scales are normal in fp32)
+                const float cap = fmaxf(__uint_as_float(up), vcap);
+                const float down = vcap / cap, by = (float)((int)(__float_as_uint(cap) >> 23) - 127) - vexp;
+                vcap = cap;
+                vexp += by;
+                p_top = kTopP / cap;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    m_run[rb] += by;
+                    lsum[rb] *= down;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[rb][t] *= down;
+                }
+            }
             float pf[SG][8], bs[SG];
             auto exps = [&](int i) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
-                    const float s = p.scale_log2;
-                    const f4 ks = SCALED ? scale4(kt, false) : f4{s, s, s, s};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) pf[i][4 * kt + r] = fmaf(sc[i][kt][r], ks[r], -m_run[r0 + i]);
+                    for (int r = 0; r < 4; ++r)
+                        pf[i][4 * kt + r] = fmaf(sc[i][kt][r], SCALED ? ks[kt][r] : p.scale_log2, -m_run[r0 + i]);
                 }
                 if (masked) {
                     uint32_t w = seen(r0 + i);
@@ -538,10 +540,9 @@ __global__ __launch_bounds__(64 * WR, RB == 1 && D <= 80 ? 3 : 2) void tree_kern
                     const uint32_t w = masked ? seen(rb) : ~0u;
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt) {
-                        const float s = p.scale_log2;
-                        const f4 ks = SCALED ? scale4(kt, false) : f4{s, s, s, s};
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) ml = vmax(ml, seen_or_inf(sc[i][kt][r] * ks[r], w, 16 * kt + r));
+                        for (int r = 0; r < 4; ++r)
+                            ml = vmax(ml, seen_or_inf(sc[i][kt][r] * (SCALED ? ks[kt][r] : p.scale_log2), w, 16 * kt + r));
                     }
                     ml = max_over_groups(ml);
                     if constexpr (SCALED) ml += vexp;
