@@ -25,11 +25,11 @@
 // (P <= 2^15), so that the low part of a P of 2^-16 of the row's largest still
 // has 19 bits; it moves when a row's largest score grows by more than 2^4.
 // What bounds it, 64 heads over 8 kv heads of 80: 16 nodes on 32 fp16 sequences
-// of 128..4096 take 84 us, of which the bytes alone are 49 (173 MB by the ring
-// without products) and the merge 12; 64 nodes on 8 FP8 sequences of 8000..16384
-// take 250 us, of which the products (three per key and row: S, P's high and low
-// part) are 108 at a large matrix product's rate, and the rest the softmax and
-// the widening on the vector units beside them.
+// of 128..4096 take 76 us, of which the ring without products takes 49 (210 MB)
+// and the merge 12; 64 nodes on 8 FP8 sequences of 8000..16384 take 233 us, of
+// which the products (three per key and row: S, P's high and low part) are 108
+// at a large matrix product's rate, and the rest the softmax and the widening on
+// the vector units beside them.
 // int8 pages: K and V are exact fp16 integers; the key's K scale multiplies
 // the score, its V scale P (whose exponent is lowered by a running power of two
 // at or above the scales, so that any scale keeps the product in range).
