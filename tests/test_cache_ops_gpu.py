@@ -237,7 +237,7 @@ def some_scores(S, hkv, n, seed=0):
 
 @pytest.mark.parametrize("lens,budget", [
     ([1], 1), ([2], 1), ([63, 64, 65], 64), ([64, 65, 66, 130], 63), ([255, 256, 257], 255), ([100, 5, 0, 64], 32),
-    ([1000, 700, 1], 999), ([2049, 2050, 2064, 2048], 2048), ([4096, 4097, 3000], 500), ([9000, 4097], 4096)])
+    ([1000, 700, 1], 999), ([1024], 700), ([1025], 700), ([2049, 2050, 2064, 2048], 2048), ([4096, 4097, 3000], 500), ([9000, 4097], 4096)])
 def test_plan_lengths(lens, budget):
     check_plan(some_scores(len(lens), 3, max(lens) + 5), lens, budget)
 
