@@ -23,7 +23,9 @@ namespace {
 // at a time, and only the waves' totals meet in LDS.
 //
 // Rows of up to 32768 slots (evict_plan_kernel) keep their keys in LDS; longer
-// ones (evict_plan_long_kernel) read them again for every pass.
+// ones (evict_plan_long_kernel) read them again for every pass.  What bounds it
+// is the chain of passes with a barrier each: 512 rows of 2064 slots 9.7 us, 32
+// rows of 16384 18.8.
 
 constexpr int kPlanLdsKeys = 32768;
 
@@ -404,7 +406,9 @@ __device__ __forceinline__ bool place(const RowMoveParams& p, const int32_t* tab
 }
 
 // A thread moves one 16-byte piece of one row: sources and targets of a plan
-// are disjoint, so the moves need no order.
+// are disjoint, so the moves need no order.  Bound by the lines it touches: a
+// head's fp16 row of 80 is 160 bytes at any place, 2 or 3 lines of 128 each way
+// (4 prompts cut to 4096 rows, 53 MB: 18 us where whole lines would take 10).
 __global__ __launch_bounds__(256) void evict_apply_kernel(RowMoveParams p) {
     const int s = blockIdx.y / p.num_kv_heads, h = blockIdx.y - s * p.num_kv_heads;
     const int pieces = p.row_bytes / 16, per = 2 * pieces;  // K's, then V's
@@ -434,7 +438,8 @@ __global__ __launch_bounds__(256) void evict_apply_kernel(RowMoveParams p) {
 
 // A workgroup owns a column slice of one layer's K or V rows of one sequence,
 // and holds every accepted row's slice in registers before it writes any:
-// sources may be other rows' targets.
+// sources may be other rows' targets.  One round trip: 64 layers of one
+// sequence 4.0 us, 16 layers of 32 (8 rows each) 8.6 us.
 constexpr int kCommitRegs = 8;
 constexpr int kCommitItems = 256 * kCommitRegs;
 
